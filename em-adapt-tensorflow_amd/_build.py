@@ -20,7 +20,10 @@ ABLATE_LIB_PATH = os.path.join(PKG_DIR, "libemadapt_hip_ablate.so")
 ARCH = "gfx950"
 # No -ffast-math: the E-step must keep IEEE fp32 semantics (bit-exact label maps), and the conv
 # accumulation order is part of the documented numerics.
-CXXFLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH, "-Wall", "-Wno-unused-function"]
+# No packed fp32 instructions: some forms of v_pk_{add,mul,fma}_f32, which -O3 makes from ordinary float code, have given wrong results on
+# this hardware now and then, without an error.  (hipcc's host pass warns that it does not know the feature: harmless.)
+CXXFLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH, "-Wall", "-Wno-unused-function", "-Xclang", "-target-feature", "-Xclang",
+            "-packed-fp32-ops"]
 
 
 def _hipcc():
