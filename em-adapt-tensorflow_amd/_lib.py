@@ -46,6 +46,12 @@ class VocSample(ctypes.Structure):
                 ("h1", ctypes.c_int32), ("w1", ctypes.c_int32), ("flip", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
+class AdamwTensor(ctypes.Structure):
+    """Mirror of emadapt_adamw_tensor (include/emadapt.h)."""
+    _fields_ = [("w", c_void_p), ("g", c_void_p), ("m", c_void_p), ("v", c_void_p), ("e", c_void_p), ("n", c_int64), ("unit", c_int64),
+                ("weight_decay", c_float), ("lr_scale", c_float)]
+
+
 class ConvDesc(ctypes.Structure):
     """Mirror of emadapt_conv_desc (include/emadapt.h)."""
 
@@ -150,6 +156,23 @@ PROTOTYPES = {
     "emadapt_sgd_accumulate_pack": (c_int, [_vp, _vp, c_int64, c_int64, c_float, c_float, _vp, c_int, _vp]),
     "emadapt_grad_pack": (c_int, [_vp, c_int64, _vp, c_int, c_int64, _vp]),
     "emadapt_grad_owner_sum": (c_int, [_vp, c_int, c_int, c_int64, _vp, _vp]),
+    "emadapt_label_logp_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "emadapt_label_logp": (c_int, [_vp, c_int, c_int64, _vp, c_int64, c_int64, _vp, _vp, _vp, c_size_t, _vp]),
+    "emadapt_label_logp_bwd": (c_int, [_vp, c_int, c_int64, _vp, _vp, _vp, c_int64, c_int64, _vp, c_int, _vp]),
+    "emadapt_policy_loss_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "emadapt_policy_loss": (c_int, [_vp, c_int, c_int64, _vp, _vp, _vp, _vp, _vp, c_int64, c_int64, c_double, c_double, c_float, c_float, _vp,
+                                    _vp, _vp, c_int, _vp, c_size_t, _vp]),
+    "emadapt_preference_loss_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "emadapt_preference_loss": (c_int, [_vp, c_int, c_int64, _vp, _vp, c_int64, _vp, c_int64, c_int64, c_float, c_float, c_float, _vp, _vp, _vp,
+                                        c_int, _vp, c_size_t, _vp]),
+    "emadapt_adamw_chunks": (c_int64, [c_int, POINTER(AdamwTensor)]),
+    "emadapt_adamw_table_bytes": (c_size_t, [c_int64]),
+    "emadapt_adamw_control_bytes": (c_size_t, []),
+    "emadapt_adamw_table": (c_int, [c_int, POINTER(AdamwTensor), c_int, c_int, _vp, c_size_t]),
+    "emadapt_adamw_step": (c_int, [_vp, c_int64, c_int, c_int, _vp, c_size_t, c_double, c_double, c_double, c_double, c_float, c_double,
+                                   ctypes.c_uint, c_int, _vp]),
+    "emadapt_adamw_unpack": (c_int, [_vp, _vp, _vp, c_int64, _vp, _vp, c_int, _vp]),
+    "emadapt_adamw_pack": (c_int, [_vp, _vp, c_int64, _vp, _vp, _vp, _vp]),
     "emadapt_status_word": (c_int, [POINTER(_vp)]),
     "emadapt_status_poll": (c_int, [POINTER(ctypes.c_uint), c_int, _vp]),
     "emadapt_status_collective": (c_int, [c_int]),

@@ -76,6 +76,39 @@ __device__ __forceinline__ void status_raise(unsigned *status, unsigned bits) {
     if (status) __hip_atomic_fetch_or(status, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// ---- the counter-based random generator: a function of (seed, unit) alone; dropout (igemm_common.h, where the form is explained) and the
+// stochastic rounding of the 8-bit optimiser states (adamw.hip) draw from it.  drop_key() is the part that depends on
+// the seed alone.
+__device__ __forceinline__ unsigned fmix32(unsigned h) {
+    h ^= h >> 16;
+    h *= 0x85EBCA6Bu;
+    h ^= h >> 13;
+    h *= 0xC2B2AE35u;
+    h ^= h >> 16;
+    return h;
+}
+struct DropKey { unsigned s1, s2; };
+__device__ __forceinline__ DropKey drop_key(unsigned long long seed) {
+    DropKey k;
+    k.s1 = fmix32((unsigned)seed ^ fmix32((unsigned)(seed >> 32) + 0x9E3779B9u));
+    k.s2 = fmix32(k.s1 + 0x7F4A7C15u);
+    return k;
+}
+__device__ __forceinline__ unsigned drop_hash(DropKey k, unsigned long long unit) {
+    unsigned h = (unsigned)unit * 0x9E3779B1u;
+    const unsigned hi = (unsigned)(unit >> 32);
+    if (__builtin_expect(hi != 0u, 0)) h += hi * 0x27D4EB2Fu;   // (tensors of 2^32 units and more: a branch the waves of a launch all skip)
+    h ^= k.s1;
+    h ^= h >> 15;
+    h *= 0x2C1B3C6Du;
+    h += k.s2;
+    h ^= h >> 12;
+    h *= 0x297A2D39u;
+    h ^= h >> 15;
+    return h;
+}
+__device__ __forceinline__ unsigned drop_hash(unsigned long long seed, unsigned long long unit) { return drop_hash(drop_key(seed), unit); }
+
 // ---- per-kernel event timing (bench.py roofline; see emadapt_prof_* in emadapt.h) ----
 struct ProfScope {
     ProfScope(int kind, double flops, double bytes, hipStream_t stream);

@@ -108,29 +108,7 @@ __device__ __forceinline__ float4 buf_ld4(__amdgpu_buffer_rsrc_t r, unsigned byt
 // commute with the multiplies, so no seed's stream is a shifted copy of another's -- scripts/dropout_quality.py checks the cross-seed
 // correlation, the keep rate, lag correlations along channels and pixels and the joint distribution of a quad's / an octet's
 // decisions).
-__device__ __forceinline__ unsigned fmix32(unsigned h) {
-    h ^= h >> 16;
-    h *= 0x85EBCA6Bu;
-    h ^= h >> 13;
-    h *= 0xC2B2AE35u;
-    h ^= h >> 16;
-    return h;
-}
-__device__ __forceinline__ unsigned drop_hash(unsigned long long seed, unsigned long long unit) {
-    const unsigned s1 = fmix32((unsigned)seed ^ fmix32((unsigned)(seed >> 32) + 0x9E3779B9u));
-    const unsigned s2 = fmix32(s1 + 0x7F4A7C15u);
-    unsigned h = (unsigned)unit * 0x9E3779B1u;
-    const unsigned hi = (unsigned)(unit >> 32);
-    if (__builtin_expect(hi != 0u, 0)) h += hi * 0x27D4EB2Fu;   // (tensors of 2^32 units and more: a branch the waves of a launch all skip)
-    h ^= s1;
-    h ^= h >> 15;
-    h *= 0x2C1B3C6Du;
-    h += s2;
-    h ^= h >> 12;
-    h *= 0x297A2D39u;
-    h ^= h >> 15;
-    return h;
-}
+// (fmix32, drop_hash: common.h -- the 8-bit optimiser states draw their roundings from the same hash)
 __device__ __forceinline__ bool dropout_keep(unsigned long long seed, unsigned long long idx, float keep, int keep8) {
     if (keep8) return (int)((drop_hash(seed, idx >> 2) >> (8u * ((unsigned)idx & 3u))) & 0xFFu) < keep8;
     const unsigned h = drop_hash(seed, idx >> 1);

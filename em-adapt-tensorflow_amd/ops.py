@@ -4,6 +4,7 @@ torch provides device memory and the current HIP stream; every computation happe
 libemadapt_hip.so.  All tensors are fp32, NHWC, contiguous; filters are HWIO like the reference's
 ``tf.get_variable`` shapes (deeplab.py:131-149).
 """
+import contextlib
 import ctypes
 
 import torch
@@ -826,6 +827,296 @@ def grad_owner_sum(recv, world, out):
         raise ValueError("recv must be [world x shard] of out's type")
     _lib.call("emadapt_grad_owner_sum", _p(recv), dt, int(world), out.numel(), _p(out), _stream())
     return out
+
+
+# ---- losses over the log-probability of given labels (include/emadapt.h, "Losses over the log-probability ...")
+def _rows(logits, labels, num_classes, name="labels"):
+    """Checks logits [..., ldl] f32 / bf16 with labels int64 [...]; returns (dtype code, ldl, rows)."""
+    dt = _float_dt(logits, "logits")
+    _check(labels, torch.int64, name)
+    if logits.dim() < 1:
+        raise ValueError("logits must be [..., classes]")
+    ldl = logits.shape[-1]
+    if not 0 < int(num_classes) <= ldl:
+        raise ValueError("num_classes %d does not fit logits of %d columns" % (num_classes, ldl))
+    M = labels.numel()
+    if tuple(labels.shape) != tuple(logits.shape[:-1]):
+        raise ValueError("%s has shape %s, the logits' rows %s" % (name, tuple(labels.shape), tuple(logits.shape[:-1])))
+    _same_device(logits, labels, name)
+    return dt, ldl, M
+
+
+def _float_dt(t, name):
+    """EMADAPT_DT_* of a contiguous f32 / bf16 GPU tensor of any shape."""
+    if not t.is_cuda:
+        raise ValueError("%s must live on the GPU (there is no CPU path)" % name)
+    dt = DT_F32 if t.dtype == torch.float32 else DT_BF16 if t.dtype == torch.bfloat16 else None
+    if dt is None:
+        raise TypeError("%s must be float32 or bfloat16, got %s" % (name, t.dtype))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)
+    return dt
+
+
+def _same_device(a, b, name):
+    if b.device != a.device:
+        raise ValueError("%s lives on %s, the logits on %s" % (name, b.device, a.device))
+
+
+def _row_vector(t, logits, M, name):
+    """An f32 value per row (or None)."""
+    if t is not None:
+        _check(t, name=name)
+        if t.numel() != M:
+            raise ValueError("%s holds %d values, the logits %d rows" % (name, t.numel(), M))
+        _same_device(logits, t, name)
+
+
+def _dlogits(logits, dlogits):
+    if dlogits is None:
+        return torch.empty_like(logits), _float_dt(logits, "dlogits")
+    ddt = _float_dt(dlogits, "dlogits")
+    if dlogits.shape != logits.shape:
+        raise ValueError("dlogits must have the logits' shape")
+    _same_device(logits, dlogits, "dlogits")
+    return dlogits, ddt
+
+
+def _scratch(nbytes, t):
+    """Workspace of one call, from torch's allocator (not the shared one): calls on several streams and captured graphs never share it."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
+
+
+def _on(t):
+    """The launches go to the tensors' device, whichever is current."""
+    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def label_logp(logits, labels, num_classes):
+    """(logp f32 [...], lse f32 [...]): log-probability of the given labels and the rows' log-sum-exp.  logits f32 / bf16 [..., ldl], labels
+    int64 [...]; a label outside [0, num_classes) has logp 0."""
+    dt, ldl, M = _rows(logits, labels, num_classes)
+    with _on(logits):
+        logp = torch.empty(labels.shape, dtype=torch.float32, device=logits.device)
+        lse = torch.empty_like(logp)
+        ws = _scratch(_lib.load().emadapt_label_logp_workspace_bytes(M, int(num_classes)), logits)
+        _lib.call("emadapt_label_logp", _p(logits), dt, ldl, _p(labels), M, int(num_classes), _p(logp), _p(lse), _p(ws),
+                  0 if ws is None else ws.numel(), _stream())
+    return logp, lse
+
+
+def label_logp_bwd(logits, labels, lse, dlogp, num_classes, dlogits=None):
+    """d loss / d logits from d loss / d logp and the lse of label_logp: ([c = label] - softmax) * dlogp, 0 in rows without a label and in the
+    padding columns.  dlogits: f32 / bf16 output of the logits' shape (default: their type); it must not overlap the logits."""
+    dt, ldl, M = _rows(logits, labels, num_classes)
+    _row_vector(lse, logits, M, "lse")
+    _row_vector(dlogp, logits, M, "dlogp")
+    with _on(logits):
+        dlogits, ddt = _dlogits(logits, dlogits)
+        _lib.call("emadapt_label_logp_bwd", _p(logits), dt, ldl, _p(labels), _p(lse), _p(dlogp), M, int(num_classes), _p(dlogits), ddt, _stream())
+    return dlogits
+
+
+def policy_loss(logits, actions, old_logp, advantages, num_classes, ref_logp=None, weights=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0,
+                grad_scale=None, want_grad=True, dlogits=None):
+    """The clipped policy loss with a KL term (include/emadapt.h, emadapt_policy_loss) of sampled actions int64 [...] under logits [..., ldl].
+
+    old_logp, advantages, ref_logp, weights: f32 [...] (the last two optional).  Returns (sums f32 [4], logp f32 [...], dlogits or None); sums =
+    weighted sums over the rows of the loss, its surrogate part, its KL part, and the rows whose ratio the clip holds; dlogits = grad_scale (default
+    1 / rows) times the gradient of sums[0]."""
+    dt, ldl, M = _rows(logits, actions, num_classes, "actions")
+    for t, name in ((old_logp, "old_logp"), (advantages, "advantages"), (ref_logp, "ref_logp"), (weights, "weights")):
+        _row_vector(t, logits, M, name)
+    if old_logp is None or advantages is None:
+        raise ValueError("old_logp and advantages are needed")
+    if not 0.0 <= clip_low <= 1.0 or not clip_high >= 0.0:
+        raise ValueError("clip_low must be in [0, 1] and clip_high >= 0, got %r and %r" % (clip_low, clip_high))
+    if ref_logp is None and kl_coef != 0.0:
+        raise ValueError("a KL term needs ref_logp")
+    if grad_scale is None:
+        grad_scale = 1.0 / max(M, 1)
+    with _on(logits):
+        ddt = DT_F32
+        if want_grad:
+            dlogits, ddt = _dlogits(logits, dlogits)
+        sums = torch.empty(4, dtype=torch.float32, device=logits.device)
+        logp = torch.empty(actions.shape, dtype=torch.float32, device=logits.device)
+        ws = _scratch(_lib.load().emadapt_policy_loss_workspace_bytes(M, int(num_classes)), logits)
+        _lib.call("emadapt_policy_loss", _p(logits), dt, ldl, _p(actions), _p(old_logp), _p(ref_logp), _p(advantages), _p(weights), M, int(num_classes),
+                  float(clip_low), float(clip_high), float(kl_coef), float(grad_scale), _p(sums), _p(logp), _p(dlogits) if want_grad else None, ddt,
+                  _p(ws), ws.numel(), _stream())
+    return sums, logp, (dlogits if want_grad else None)
+
+
+def preference_loss(logits, labels, seq_start, ref_logp, num_classes, beta=0.1, label_smoothing=0.0, grad_scale=None, want_grad=True, dlogits=None):
+    """The preference loss of paired sequences of rows (include/emadapt.h, emadapt_preference_loss): logits [..., ldl], labels int64 [...],
+    seq_start int64 [2 * pairs + 1] on the GPU (sequence 2j the chosen, 2j + 1 the rejected one of pair j, over the flattened rows), ref_logp f32
+    [2 * pairs] the reference model's sequence log-probabilities.
+
+    Returns (loss f32 [pairs], seq_logp f32 [2 * pairs], dlogits or None); dlogits = grad_scale (default 1 / pairs) times the gradient of loss.sum()."""
+    dt, ldl, M = _rows(logits, labels, num_classes)
+    _check(seq_start, torch.int64, "seq_start")
+    _same_device(logits, seq_start, "seq_start")
+    if seq_start.dim() != 1 or seq_start.numel() % 2 != 1:
+        raise ValueError("seq_start must hold 2 * pairs + 1 starts, got shape %s" % (tuple(seq_start.shape),))
+    pairs = seq_start.numel() // 2
+    _check(ref_logp, name="ref_logp")
+    _same_device(logits, ref_logp, "ref_logp")
+    if ref_logp.numel() != 2 * pairs:
+        raise ValueError("ref_logp must hold a value per sequence (%d), got %d" % (2 * pairs, ref_logp.numel()))
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError("label_smoothing must be in [0, 1], got %r" % label_smoothing)
+    if grad_scale is None:
+        grad_scale = 1.0 / max(pairs, 1)
+    with _on(logits):
+        ddt = DT_F32
+        if want_grad:
+            dlogits, ddt = _dlogits(logits, dlogits)
+        loss = torch.empty(pairs, dtype=torch.float32, device=logits.device)
+        seq_logp = torch.empty(2 * pairs, dtype=torch.float32, device=logits.device)
+        ws = _scratch(_lib.load().emadapt_preference_loss_workspace_bytes(M, int(num_classes)), logits)
+        _lib.call("emadapt_preference_loss", _p(logits), dt, ldl, _p(labels), _p(seq_start), pairs, _p(ref_logp), M, int(num_classes), float(beta),
+                  float(label_smoothing), float(grad_scale), _p(loss), _p(seq_logp), _p(dlogits) if want_grad else None, ddt, _p(ws),
+                  0 if ws is None else ws.numel(), _stream())
+    return loss, seq_logp, (dlogits if want_grad else None)
+
+
+ADAMW_STATES = {"f32": 0, "u8": 1}   # EMADAPT_ADAMW_*
+_ADAMW_ALIGN = 256   # every tensor's states start at a multiple of this many elements of the state buffers
+
+
+class AdamW:
+    """AdamW over a list of tensors, one launch for all of them (include/emadapt.h, "AdamW over many tensors").
+
+    params: contiguous f32 GPU tensors; grads: as many of their sizes, all f32 or all bf16; both are updated / read in place by step(), so they have to
+    live as long as this object (it holds them).  weight_decay, lr_scale: a number, or one per tensor.  state: "f32" (m, v in 32 bits) or "u8" (8-bit
+    codes, stochastic rounding from `seed`).
+
+    State buffers (tensor k's elements at offsets[k], the gaps between are zero): m, v f32 for "f32"; m8, u8 uint8 codes and powers uint8 [n / 64, 2] for
+    "u8", with unpack() / pack() between codes and values.  steps: int64 [1] on the device, the steps taken; grad_norm: f32 [1], the gradients' norm of the
+    last step that was given a max_norm."""
+
+    def __init__(self, params, grads, state="f32", betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, lr_scale=1.0, seed=0):
+        params, grads = list(params), list(grads)
+        if not params:
+            raise ValueError("no tensors to optimise")
+        if state not in ADAMW_STATES:
+            raise ValueError("state must be 'f32' or 'u8', got %r" % (state,))
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError("betas must be in [0, 1), got %r" % (betas,))
+        if not eps >= 1e-30:
+            raise ValueError("eps must be at least 1e-30, got %r" % (eps,))
+        for k, p in enumerate(params):
+            _check(p, name="params[%d]" % k)
+            if p.device != params[0].device:
+                raise ValueError("params[%d] lives on %s, params[0] on %s" % (k, p.device, params[0].device))
+        _refuse_overlap(params, "params")
+        self.params, self.state, self.betas, self.eps, self.seed = params, state, (float(betas[0]), float(betas[1])), float(eps), int(seed) & 0xFFFFFFFF
+        self.device = params[0].device
+        self._wd = _per_tensor(weight_decay, len(params), "weight_decay")
+        self._ls = _per_tensor(lr_scale, len(params), "lr_scale")
+        self.offsets, total = [], 0
+        for p in params:
+            self.offsets.append(total)
+            total += (p.numel() + _ADAMW_ALIGN - 1) // _ADAMW_ALIGN * _ADAMW_ALIGN
+        self.total = total
+        if state == "f32":
+            self.m = torch.zeros(total, dtype=torch.float32, device=self.device)
+            self.v = torch.zeros(total, dtype=torch.float32, device=self.device)
+        else:
+            self.m8 = torch.zeros(total, dtype=torch.uint8, device=self.device)
+            self.u8 = torch.zeros(total, dtype=torch.uint8, device=self.device)
+            self.powers = torch.zeros((total // 64, 2), dtype=torch.uint8, device=self.device)
+        lib = _lib.load()
+        self._control = torch.zeros(lib.emadapt_adamw_control_bytes(), dtype=torch.uint8, device=self.device)
+        self.steps = self._control[:8].view(torch.int64)
+        self.grad_norm = self._control[8:12].view(torch.float32)
+        self._step = lib.emadapt_adamw_step
+        self.set_grads(grads)
+
+    def set_grads(self, grads):
+        """The gradients that step() reads from now on (a copy of their addresses goes to the device; not under graph capture)."""
+        grads = list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError("%d gradients for %d tensors" % (len(grads), len(self.params)))
+        dt = _float_dt(grads[0], "grads[0]")
+        arr = (_lib.AdamwTensor * len(grads))()
+        size = 1 if self.state == "u8" else 4
+        m, v = (self.m8, self.u8) if self.state == "u8" else (self.m, self.v)
+        for k, (p, g) in enumerate(zip(self.params, grads)):
+            if _float_dt(g, "grads[%d]" % k) != dt:
+                raise TypeError("the gradients must have one type, got %s and %s" % (grads[0].dtype, g.dtype))
+            if g.numel() != p.numel():
+                raise ValueError("grads[%d] holds %d elements, the tensor %d" % (k, g.numel(), p.numel()))
+            if g.device != self.device:
+                raise ValueError("grads[%d] lives on %s, the tensors on %s" % (k, g.device, self.device))
+            off = self.offsets[k]
+            arr[k].w, arr[k].g, arr[k].n, arr[k].unit = p.data_ptr(), g.data_ptr(), p.numel(), off
+            arr[k].m, arr[k].v = m.data_ptr() + off * size, v.data_ptr() + off * size
+            arr[k].e = self.powers.data_ptr() + off // 64 * 2 if self.state == "u8" else None
+            arr[k].weight_decay, arr[k].lr_scale = self._wd[k], self._ls[k]
+        lib = _lib.load()
+        chunks = lib.emadapt_adamw_chunks(len(grads), arr)
+        if chunks < 0:
+            raise _lib.EmadaptError(int(chunks), "emadapt_adamw_chunks")
+        host = torch.zeros(lib.emadapt_adamw_table_bytes(chunks), dtype=torch.uint8)
+        _lib.call("emadapt_adamw_table", len(grads), arr, dt, ADAMW_STATES[self.state], ctypes.c_void_p(host.data_ptr()), host.numel())
+        self.grads, self._gdt, self._chunks = grads, dt, chunks
+        self._grads_apart = None
+        with _on(self._control):
+            self._table = host.to(self.device)
+
+    def step(self, lr, grad_scale=1.0, max_norm=0.0, zero_grads=False):
+        """One step: gradients times grad_scale, held to the global norm max_norm (0: not), weights and moments updated in place.  zero_grads: the
+        gradients are zeroed behind it.  A gradient (or norm) that is not finite leaves its elements (or the whole step) out and raises
+        STATUS_NAN_GRADIENT of the device status word; while the word is raised the step does nothing (status_poll)."""
+        if zero_grads and not self._grads_apart:
+            _refuse_overlap(self.grads, "grads")
+            self._grads_apart = True
+        with _on(self._control):
+            rc = self._step(self._table.data_ptr(), self._chunks, self._gdt, ADAMW_STATES[self.state], self._control.data_ptr(), self._control.numel(),
+                            float(lr), self.betas[0], self.betas[1], self.eps, float(grad_scale), float(max_norm), self.seed, 1 if zero_grads else 0,
+                            torch.cuda.current_stream().cuda_stream)
+        if rc:
+            raise _lib.EmadaptError(rc, "emadapt_adamw_step")
+
+    def unpack(self, dtype=torch.float32):
+        """(m, u) of the 8-bit states as flat tensors of values (exact in float32 and bfloat16); u is the root of the second moment."""
+        if self.state != "u8":
+            raise ValueError("unpack() is for 8-bit states; m and v of 32-bit states are there as they are")
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError("states unpack to float32 or bfloat16, got %s" % dtype)
+        with _on(self._control):
+            m = torch.empty(self.total, dtype=dtype, device=self.device)
+            u = torch.empty(self.total, dtype=dtype, device=self.device)
+            _lib.call("emadapt_adamw_unpack", _p(self.m8), _p(self.u8), _p(self.powers), self.total, _p(m), _p(u),
+                      DT_BF16 if dtype == torch.bfloat16 else DT_F32, _stream())
+        return m, u
+
+    def pack(self, m, u):
+        """Set the 8-bit states from flat f32 values (rounded to nearest; exact for what unpack() gives)."""
+        if self.state != "u8":
+            raise ValueError("pack() is for 8-bit states")
+        for t, name in ((m, "m"), (u, "u")):
+            _check(t, name=name)
+            if t.numel() != self.total or t.device != self.device:
+                raise ValueError("%s must hold the %d elements of the state buffers on %s" % (name, self.total, self.device))
+        with _on(self._control):
+            _lib.call("emadapt_adamw_pack", _p(m), _p(u), self.total, _p(self.m8), _p(self.u8), _p(self.powers), _stream())
+
+
+def _per_tensor(v, n, name):
+    v = [float(v)] * n if isinstance(v, (int, float)) else [float(x) for x in v]
+    if len(v) != n:
+        raise ValueError("%s holds %d values for %d tensors" % (name, len(v), n))
+    return v
+
+
+def _refuse_overlap(tensors, name):
+    spans = sorted((t.data_ptr(), t.numel() * t.element_size(), k) for k, t in enumerate(tensors) if t.numel())
+    for (a, n, i), (b, _, j) in zip(spans, spans[1:]):
+        if a + n > b:
+            raise ValueError("%s[%d] and %s[%d] share memory" % (name, i, name, j))
 
 
 def status_word():

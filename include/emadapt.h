@@ -68,8 +68,10 @@ extern "C" {
  *        emadapt_sgd_momentum_payload_tiles: the optimizer pass of a layer that also writes the layer's two tiled bf16 filter images; emadapt_sgd_accumulate_momentum_multi: the pass
  *        over several layers' segments in one launch; emadapt_weights_to_bf16_multi: several filters' bf16 images in one launch.
  *   206  round 6, added: emadapt_voc_preprocess (the input pipeline of a batch in one launch), emadapt_host_register / _unregister / emadapt_memcpy_h2d_async; emadapt_status_raise; emadapt_status_collective (data-parallel jobs: the failure travels with the exchanged gradient instead of
- *        being decided from each rank's own word), EMADAPT_STATUS_NAN_GRADIENT. */
-#define EMADAPT_ABI_VERSION 206
+ *        being decided from each rank's own word), EMADAPT_STATUS_NAN_GRADIENT.
+ *   207  added: emadapt_label_logp (+ _bwd), emadapt_policy_loss, emadapt_preference_loss (+ _workspace_bytes); emadapt_adamw_* (AdamW over
+ *        many tensors, moments in 32 or 8 bits, global gradient norm). */
+#define EMADAPT_ABI_VERSION 207
 int emadapt_version(void);
 const char *emadapt_strerror(int code);
 int emadapt_last_hip_error(void);          /* hipError_t of the last failing HIP call on this thread */
@@ -539,6 +541,91 @@ int emadapt_sgd_momentum_payload(float *w, float *v, float *accum, const void *p
  * emadapt_sgd_accumulate leaves in a zeroed accumulator and emadapt_grad_pack then rounds, without the accumulator (dist.py `prepacked`). */
 int emadapt_sgd_accumulate_pack(const float *g, const float *w, int64_t n, int64_t n_decay, float weight_decay, float scale,
                                 void *dst, int dst_dtype, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Losses over the log-probability of given labels (ABI 207): what trains on rewards or on preferences instead of on a label map.
+ * They stand beside emadapt_softmax_ce and hand the backward pass the same thing, d loss / d logits in the padded row layout.
+ *   logits   f32 or bf16 (dtype = EMADAPT_DT_*), rows of ldl >= C elements of which the first C count; any element alignment
+ *   labels   int64 [M]; a label outside [0, C) (a void pixel, a prompt token) takes its row out: log-probability 0, gradient 0,
+ *            whatever the row's logits hold (infinities and NaN included)
+ *   dlogits  f32 or bf16 [M][ldl], written as a whole: the padding columns and the rows that take no part become 0.  It must not
+ *            overlap the logits (EMADAPT_ERR_INVALID)
+ * A logit of -inf is a class of probability 0.  Arithmetic is f32, sums over rows f64 in a fixed order: results are bit-identical from
+ * run to run.  The reference has no counterpart (its one loss is the cross-entropy of deeplab.py:182).
+ * ---------------------------------------------------------------------------------------- */
+
+/* lse[r] = log sum_{c < C} exp(logits[r][c]);  logp[r] = logits[r][labels[r]] - lse[r].  Either output may be NULL. */
+size_t emadapt_label_logp_workspace_bytes(int64_t M, int64_t C);
+int emadapt_label_logp(const void *logits, int dtype, int64_t ldl, const int64_t *labels, int64_t M, int64_t C, float *logp, float *lse,
+                       void *workspace, size_t workspace_bytes, void *stream);
+/* dlogits[r][c] = ([c == labels[r]] - exp(logits[r][c] - lse[r])) * dlogp[r]; a row with dlogp 0 is 0. */
+int emadapt_label_logp_bwd(const void *logits, int dtype, int64_t ldl, const int64_t *labels, const float *lse, const float *dlogp,
+                           int64_t M, int64_t C, void *dlogits, int dlogits_dtype, void *stream);
+
+/* The clipped policy loss with a KL term.  Per row, with ratio = exp(logp - old_logp), q = ref_logp - logp:
+ *   surrogate = max(-A ratio, -A clamp(ratio, 1 - clip_low, 1 + clip_high))        kl = exp(q) - q - 1   (0 when ref_logp is NULL)
+ *   sums[4] = sum w (surrogate + kl_coef kl), sum w surrogate, sum w kl, sum w [the clip holds]
+ *   dlogits = grad_scale * d sums[0] / d logits
+ * weights f32 [M] or NULL (all 1); weight 0 takes the row out like a label outside [0, C).  Whether the clip holds is decided as
+ * exact arithmetic on the inputs decides it (rows within rounding of a border are looked at in 64 bits).  clip_low in [0, 1],
+ * clip_high >= 0.  logp f32 [M] is an output; dlogits may be NULL (the sums and logp alone). */
+size_t emadapt_policy_loss_workspace_bytes(int64_t M, int64_t C);
+int emadapt_policy_loss(const void *logits, int dtype, int64_t ldl, const int64_t *actions, const float *old_logp, const float *ref_logp,
+                        const float *advantages, const float *weights, int64_t M, int64_t C, double clip_low, double clip_high,
+                        float kl_coef, float grad_scale, float *sums, float *logp, void *dlogits, int dlogits_dtype, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
+/* The preference loss of paired sequences of rows.  Sequence s is the rows seq_start[s] .. seq_start[s + 1) (int64 [2 pairs + 1] on the
+ * device, not decreasing, within [0, M]; a sequence may be empty); sequences 2j and 2j + 1 are the chosen and the rejected one of pair j.
+ *   seq_logp[s] = sum of logp over the sequence      h_j = beta ((seq_logp[2j] - ref_logp[2j]) - (seq_logp[2j+1] - ref_logp[2j+1]))
+ *   loss[j] = (1 - label_smoothing) softplus(-h_j) + label_smoothing softplus(h_j)
+ *   dlogits = grad_scale * d (sum_j loss[j]) / d logits; rows of no sequence: 0
+ * A start outside [0, M] is taken as the nearest bound (nothing outside the rows is touched). */
+size_t emadapt_preference_loss_workspace_bytes(int64_t M, int64_t C);
+int emadapt_preference_loss(const void *logits, int dtype, int64_t ldl, const int64_t *labels, const int64_t *seq_start, int64_t pairs,
+                            const float *ref_logp, int64_t M, int64_t C, float beta, float label_smoothing, float grad_scale, float *loss,
+                            float *seq_logp, void *dlogits, int dlogits_dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * AdamW over many tensors (ABI 207), beside the Momentum entries above.  With t = steps + 1, c = grad_scale * min(1, max_norm / norm),
+ * norm = |grad_scale * all gradients| (max_norm 0: no norm is taken, c = grad_scale), and per tensor its weight_decay and lr_scale:
+ *   g = c g;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   w = (w - lr lr_scale weight_decay w) - lr / (1 - beta1^t) lr_scale * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * each product and sum rounded to f32 on its own.
+ *   EMADAPT_ADAMW_F32   m, v f32
+ *   EMADAPT_ADAMW_U8    m and sqrt(v) as 8-bit codes (sign + 4 exponent + 3 mantissa bits; 4 exponent + 4 mantissa bits) with one power of
+ *                       two each per 64 elements (byte pairs in e), rounded stochastically by the generator at (seed, step, element);
+ *                       m, v point at ceil(n / 64) * 64 codes, e at 2 * ceil(n / 64) bytes; all zero is the initial state
+ * Use: fill an array of emadapt_adamw_tensor, ask emadapt_adamw_chunks() (negative: an error code), let emadapt_adamw_table() write the table
+ * on the host, copy it to the device; zero emadapt_adamw_control_bytes() on the device.  The control block begins with int64 steps (the steps
+ * taken; a resumed run writes it) followed by f32 norm (of the last step with max_norm > 0).  The table holds the tensors' addresses: it is
+ * valid while they live.  Tensors must not overlap.  Steps read lr from the call and t from the control block, so that a captured step can be
+ * replayed; two steps on one control block belong on one stream.
+ * A raised status word makes the step a no-op (not in collective mode: the gradient carries the failure).  A norm that is not finite
+ * makes the step a no-op; an element whose moments would leave the finite numbers is left alone; both raise EMADAPT_STATUS_NAN_GRADIENT.
+ * zero_grads: the gradients are zeroed behind the step (the clean op of deeplab.py:204).  beta1, beta2 in [0, 1), eps >= 1e-30. */
+#define EMADAPT_ADAMW_F32 0
+#define EMADAPT_ADAMW_U8 1
+typedef struct emadapt_adamw_tensor {
+    float *w;
+    void *g;             /* f32 or bf16 (grad_dtype of the table and the step) */
+    void *m, *v;
+    void *e;             /* EMADAPT_ADAMW_U8 only */
+    int64_t n;
+    int64_t unit;        /* first element's place in the generator's sequence (e.g. its offset in the state buffers) */
+    float weight_decay, lr_scale;
+} emadapt_adamw_tensor;
+int64_t emadapt_adamw_chunks(int count, const emadapt_adamw_tensor *tensors);
+size_t emadapt_adamw_table_bytes(int64_t chunks);
+size_t emadapt_adamw_control_bytes(void);
+int emadapt_adamw_table(int count, const emadapt_adamw_tensor *tensors, int grad_dtype, int state, void *table_host, size_t table_bytes);
+int emadapt_adamw_step(const void *table, int64_t chunks, int grad_dtype, int state, void *control, size_t control_bytes, double lr,
+                       double beta1, double beta2, double eps, float grad_scale, double max_norm, unsigned seed, int zero_grads,
+                       void *stream);
+/* 8-bit states <-> values (checkpoints): n a multiple of 64; u = sqrt(v).  unpack writes f32 or bf16 (exact in both); pack rounds to
+ * nearest and gives back what unpack gave. */
+int emadapt_adamw_unpack(const void *m_codes, const void *u_codes, const void *powers, int64_t n, void *m, void *u, int dtype, void *stream);
+int emadapt_adamw_pack(const float *m, const float *u, int64_t n, void *m_codes, void *u_codes, void *powers, void *stream);
 
 /* ------------------------------------------------------------------------------------------
  * Launch-plan overrides.  Every convolution picks a kernel variant and a split factor from its shape; these
