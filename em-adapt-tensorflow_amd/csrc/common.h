@@ -12,6 +12,9 @@ extern thread_local int g_last_hip_error;
 
 inline int hip_fail(hipError_t e) {
     g_last_hip_error = (int)e;
+    // (the runtime keeps a failed call's error for the next hipGetLastError(): reported here, it must not turn up as the next launch's.
+    // Seen where hipHostRegister is refused: the input pipeline went on without it and its first kernel launch "failed")
+    (void)hipGetLastError();
     return EMADAPT_ERR_HIP;
 }
 
