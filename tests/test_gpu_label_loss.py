@@ -40,7 +40,7 @@ def _reference(torch, z, labels, C, used=None):
     used = ok if used is None else ok & used
     at = x.gather(1, torch.where(ok, labels, 0)[:, None])[:, 0]
     logp = torch.where(used, at - lse, torch.zeros_like(lse))
-    fin = torch.where(torch.isinf(x), torch.zeros_like(x), x)
+    fin = torch.where(x.abs() > 1e30, torch.zeros_like(x), x)   # (masked places weigh nothing)
     n = C / (64 if C > 512 else 4) + 1
     tol = H * (n + 32 + 3 * (fin.amax(1) - fin.amin(1)) + 2 * lse.abs() + x.amax(1).abs())
     return x, lse, logp, used, tol
@@ -136,6 +136,34 @@ def test_rows_that_take_no_part_may_hold_anything(env):
         lab3[3] = -1
         loss, seq, d = ops.preference_loss(z, lab3, at, torch.zeros(2, device="cuda"), C)
         assert bool(torch.isfinite(loss).all()) and bool(torch.isfinite(seq).all()) and bool((d[:4] == 0).all()) and bool(torch.isfinite(d).all())
+
+
+@pytest.mark.parametrize("C", [21, 900, 5000, 130000, 300000])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_rows_at_the_types_lowest_and_largest_values(env, C, dtype):
+    """A mask of the type's lowest value over a part of a row, over all of it (then every class is as likely), and logits near the largest."""
+    ops, torch = env
+    z = _logits(torch, 5, C, dtype, 14)
+    lo, big = torch.finfo(z.dtype).min, torch.finfo(z.dtype).max
+    z[0] = lo
+    z[1, 1:] = lo
+    z[2, 0] = big
+    z[3, C // 2] = lo
+    z[4] = big
+    lab = torch.zeros(5, dtype=torch.int64, device="cuda")
+    logp, lse = ops.label_logp(z, lab, C)
+    sums, lp, d = ops.policy_loss(z, lab, logp - 0.1, torch.ones(5, device="cuda"), C, clip_high=10.0, grad_scale=1.0)
+    assert bool(torch.isfinite(logp).all()) and bool(torch.isfinite(d).all()) and torch.equal(lp, logp)
+    at = torch.tensor([0, 3, 5], device="cuda")
+    loss, seq, d2 = ops.preference_loss(z, lab, at, torch.zeros(2, device="cuda"), C)
+    assert bool(torch.isfinite(loss).all()) and bool(torch.isfinite(d2).all()) and bool(torch.isfinite(ops.label_logp_bwd(z, lab, lse, torch.ones(5, device="cuda"), C)).all())
+    for r in (0, 4):   # every class is as likely
+        assert abs(float(logp[r]) + np.log(C)) < 1e-5
+        ratio = -float(d[r, 0])
+        assert abs(float(d[r, 1]) * (C - 1) + float(d[r, 0])) < 0.02 * abs(ratio)
+    assert abs(float(logp[1])) < 1e-6 and abs(float(logp[2])) < 1e-6
+    x, want_lse, want, used, tol = _reference(torch, z[3:4], lab[3:4], C)
+    assert abs(float(logp[3]) - float(want[0])) < float(tol[0]) * 2
 
 
 def test_rows_that_count_keep_their_nan(env):
