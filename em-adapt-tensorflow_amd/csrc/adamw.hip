@@ -37,13 +37,13 @@ struct AdamwChunk {
     int pad;
 };
 static_assert(sizeof(AdamwChunk) == 64, "one cache line half, one uniform load");
-constexpr int kChunk = 4096, kBlock = 64, kParts = 2048;
+constexpr int kRounds = 4, kChunk = 1024 * kRounds, kBlock = 64, kParts = 2048;   // (four elements to a thread and round)
 
-// The control block on the device.  steps persists; the rest is what one step's kernels hand to the next.
+// The control block on the device: steps and norm are the caller's to read, the rest is what one step's launches hand on.
 struct AdamwControl {
     long long steps;
-    float norm, coef, rate, root2;
-    unsigned go, pad;
+    float norm, coef, rate, root2;   // of this step: the clip's factor and the bias corrections
+    unsigned go, ticket;             // whether it happens; the norm's workgroups that are done (0 between launches)
     double sum[kParts];
 };
 
@@ -54,205 +54,307 @@ struct AdamwArgs {
     int zero_grads;
 };
 
-template <typename T> __device__ __forceinline__ void load4(const T *p, float (&v)[4]);
-template <> __device__ __forceinline__ void load4<float>(const float *p, float (&v)[4]) { __builtin_memcpy(v, p, 16); }
-template <> __device__ __forceinline__ void load4<__bf16>(const __bf16 *p, float (&v)[4]) {
-    __bf16 t[4];
-    __builtin_memcpy(t, p, 8);
-#pragma unroll
-    for (int k = 0; k < 4; k++) v[k] = (float)t[k];
+// The tensors' addresses come out of memory: said to be global here, or every access would be a flat one (which waits for the LDS as well).
+#define EMADAPT_GLOBAL __attribute__((address_space(1)))
+template <typename T> __device__ __forceinline__ EMADAPT_GLOBAL T *global(void *p) { return (EMADAPT_GLOBAL T *)p; }
+
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 h4 __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ void load4(const EMADAPT_GLOBAL float *p, float (&v)[4]) {
+    const f4 t = *(const EMADAPT_GLOBAL f4 *)p;
+    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+}
+__device__ __forceinline__ void load4(const EMADAPT_GLOBAL __bf16 *p, float (&v)[4]) {
+    const h4 t = *(const EMADAPT_GLOBAL h4 *)p;
+    v[0] = (float)t.x; v[1] = (float)t.y; v[2] = (float)t.z; v[3] = (float)t.w;
+}
+__device__ __forceinline__ void zero4(EMADAPT_GLOBAL float *p) { *(EMADAPT_GLOBAL f4 *)p = f4{0.f, 0.f, 0.f, 0.f}; }
+__device__ __forceinline__ void zero4(EMADAPT_GLOBAL __bf16 *p) { *(EMADAPT_GLOBAL h4 *)p = h4{(__bf16)0.f, (__bf16)0.f, (__bf16)0.f, (__bf16)0.f}; }
+// 16 bytes that are not read again soon
+__device__ __forceinline__ void load4_once(const EMADAPT_GLOBAL float *p, float (&v)[4]) {
+    const f4 t = __builtin_nontemporal_load((const EMADAPT_GLOBAL f4 *)p);
+    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+}
+__device__ __forceinline__ void store4_once(EMADAPT_GLOBAL float *p, const float (&v)[4]) {
+    const f4 t = {v[0], v[1], v[2], v[3]};
+    __builtin_nontemporal_store(t, (EMADAPT_GLOBAL f4 *)p);
 }
 
-__device__ __forceinline__ double block_sum_f64(double v, double *sh) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double r = 0.0;
-    for (int k = 0; k < (int)(blockDim.x >> 6); k++) r += sh[k];
-    __syncthreads();
-    return r;
-}
-
-// Sum of squares of all gradients, in 64 bits: the products of 24-bit numbers are exact, so the norm and with it the clip's factor are
-// the ones of exact arithmetic whatever the split (the double adds run beside the loads).
-template <typename TG>
-__global__ void __launch_bounds__(256) adamw_norm_kernel(const AdamwChunk *__restrict__ table, long long nchunks, AdamwControl *__restrict__ ctl) {
-    __shared__ double sh[4];
-    double s = 0.0;
-    for (long long c = blockIdx.x; c < nchunks; c += gridDim.x) {
-        const TG *g = static_cast<const TG *>(table[c].g);
-        const int n = table[c].n;
-        for (int i = threadIdx.x * 4; i < n; i += 1024) {
-            float v[4];
-            if (i + 4 <= n) load4(g + i, v);
-            else
-                for (int k = 0; k < 4; k++) v[k] = i + k < n ? (float)g[i + k] : 0.f;
-            for (int k = 0; k < 4; k++) s += (double)v[k] * (double)v[k];
-        }
-    }
-    s = block_sum_f64(s, sh);
-    if (threadIdx.x == 0) ctl->sum[blockIdx.x] = s;
-}
-
-// Everything that is the same for all elements: the clip's factor, the bias corrections of step t, whether the step happens at all.
-__global__ void __launch_bounds__(256) adamw_control_kernel(AdamwControl *__restrict__ ctl, int nparts, double lr, double b1, double b2,
-                                                          float grad_scale, double max_norm, unsigned *__restrict__ status, int ignore_status) {
-    __shared__ double sh[4];
-    double s = 0.0;
-    for (int i = threadIdx.x; i < nparts; i += 256) s += ctl->sum[i];
-    s = block_sum_f64(s, sh);
-    if (threadIdx.x != 0) return;
-    bool go = ignore_status || !status_raised(status);
-    float coef = grad_scale;
-    if (nparts > 0) {
-        const double norm = fabs((double)grad_scale) * sqrt(s);
+struct AdamwScalars {
+    double lr, beta1, beta2, max_norm;
+    float grad_scale;
+    int clip, ignore_status;
+};
+// What is the same for all elements of a step, by one thread: whether it happens, the clip's factor, the bias corrections.
+__device__ void adamw_control(AdamwControl *ctl, const AdamwScalars &a, double sum, unsigned *status) {
+    bool go = a.ignore_status || !status_raised(status);
+    float coef = a.grad_scale;
+    if (a.clip) {
+        const double norm = fabs((double)a.grad_scale) * sqrt(sum);
         ctl->norm = (float)norm;
         if (!(norm <= 1.7976931348623157e308)) {
             if (go) status_raise(status, EMADAPT_STATUS_NAN_GRADIENT);
             go = false;
-        } else if (norm > max_norm) coef = (float)((double)grad_scale * (max_norm / norm));
+        } else if (norm > a.max_norm) coef = (float)((double)a.grad_scale * (a.max_norm / norm));
     }
     ctl->go = go ? 1u : 0u;
     if (!go) return;
     const long long t = ctl->steps + 1;
     ctl->steps = t;
     ctl->coef = coef;
-    ctl->rate = (float)(lr / (1.0 - pow(b1, (double)t)));
-    ctl->root2 = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
+    ctl->rate = (float)(a.lr / (1.0 - pow(a.beta1, (double)t)));
+    ctl->root2 = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)t)));
+}
+__global__ void adamw_control_kernel(AdamwControl *ctl, AdamwScalars a, unsigned *__restrict__ status) { adamw_control(ctl, a, 0.0, status); }
+
+// Sum of squares of all gradients, in 64 bits: the products of 24-bit numbers are exact, so the norm and with it the clip's factor are
+// the ones of exact arithmetic whatever the split (the double adds run beside the loads).  The last workgroup adds the parts up in their
+// order and does the control kernel's work.  The ticket is a relaxed atomic behind a wait for the part's own store: a release of every
+// workgroup writes the XCD's L2 back each time (410 -> 611 us for the step of 65.1 M parameters).  Only here, where 2048 workgroups
+// have one: they come at 3.6 ns each.
+template <typename TG>
+__global__ void __launch_bounds__(256) adamw_norm_kernel(const AdamwChunk *__restrict__ table, long long nchunks, AdamwControl *ctl, AdamwScalars a,
+                                                        unsigned *__restrict__ status) {
+    __shared__ double sh[4];
+    __shared__ bool last;
+    double s = 0.0;
+    constexpr int N = 16 / (int)sizeof(TG), kLoads = kChunk / (256 * N);   // 16 bytes to a load: 4 loads of f32, 2 of bf16
+    typedef TG Piece __attribute__((ext_vector_type(16 / sizeof(TG)), aligned(sizeof(TG))));
+    for (long long c = blockIdx.x; c < nchunks; c += gridDim.x) {
+        const EMADAPT_GLOBAL TG *g = global<TG>(table[c].g);
+        const int n = table[c].n;
+        Piece v[kLoads];
+        if (n == kChunk) {
+#pragma unroll
+            for (int q = 0; q < kLoads; q++) v[q] = *(const EMADAPT_GLOBAL Piece *)(g + (q * 256 + threadIdx.x) * N);
+        } else {
+#pragma unroll
+            for (int q = 0; q < kLoads; q++)
+#pragma unroll
+                for (int k = 0; k < N; k++) {
+                    const int i = (q * 256 + threadIdx.x) * N + k;
+                    v[q][k] = i < n ? g[i] : (TG)0.f;
+                }
+        }
+#pragma unroll
+        for (int q = 0; q < kLoads; q++)
+#pragma unroll
+            for (int k = 0; k < N; k++) s = __builtin_fma((double)(float)v[q][k], (double)(float)v[q][k], s);
+    }
+    s = block_sum_f64(s, sh);
+    if (threadIdx.x == 0) {
+        __hip_atomic_store(&ctl->sum[blockIdx.x], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __builtin_amdgcn_s_waitcnt(0);
+        last = __hip_atomic_fetch_add(&ctl->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    s = 0.0;
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) s += __hip_atomic_load(&ctl->sum[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s = block_sum_f64(s, sh);
+    if (threadIdx.x != 0) return;
+    ctl->ticket = 0u;
+    adamw_control(ctl, a, s, status);
 }
 
-// One element (m, v in, m, u, w out), every operation rounded on its own.  false: the gradient took a moment out of the finite numbers.
-__device__ __forceinline__ bool adamw_element(float g, float &m, float &v, float &u, float &w, float coef, float fade, float rate, float root2,
-                                              const AdamwArgs &a) {
+// a / b to one rounding or next to it (b a normal number of ordinary size): a reciprocal and one correction by the remainder
+__device__ __forceinline__ float quotient(float a, float b) {
+    const float r = __builtin_amdgcn_rcpf(b), q = a * r;
+    return __builtin_fmaf(__builtin_fmaf(-b, q, a), r, q);
+}
+// sqrt(x) to nearest for x >= 2^-120 (below, next to it): the instruction's value or a neighbour, by the remainders' signs
+__device__ __forceinline__ float root(float x) {
+    const float s = __builtin_amdgcn_sqrtf(x);
+    const float lo = __uint_as_float(__float_as_uint(s) - 1u), hi = __uint_as_float(__float_as_uint(s) + 1u);
+    const float t = __builtin_fmaf(-lo, s, x) <= 0.f ? lo : s;   // (0 and inf: the neighbours' remainders are NaN or 0, s stays)
+    return __builtin_fmaf(-hi, s, x) > 0.f ? hi : t;
+}
+// One element: new moments, the root of the second and the new weight, every operation rounded on its own.
+struct Element {
+    float m, v, u, w;
+};
+__device__ __forceinline__ Element adamw_element(float g, float m, float v, float w, float coef, float fade, float rate, float root2, const AdamwArgs &a) {
 #pragma clang fp contract(off)
+    Element e;
     const float gs = g * coef;
-    const float m1 = m * a.b1 + gs * a.omb1;
-    const float v1 = v * a.b2 + (gs * gs) * a.omb2;
-    const bool ok = fabsf(m1) < INFINITY && v1 < INFINITY;
-    const float u1 = sqrtf(v1);
-    const float w1 = (w - fade * w) - rate * (m1 / (u1 * root2 + a.eps));
-    m = ok ? m1 : m;
-    v = ok ? v1 : v;
-    u = ok ? u1 : u;
-    w = ok ? w1 : w;
-    return ok;
+    e.m = m * a.b1 + gs * a.omb1;
+    e.v = v * a.b2 + (gs * gs) * a.omb2;
+    e.u = root(e.v);
+    e.w = (w - fade * w) - rate * quotient(e.m, e.u * root2 + a.eps);
+    return e;
 }
+__device__ __forceinline__ bool finite(const Element &e) { return fabsf(e.m) < INFINITY && e.v < INFINITY; }
 
+// A workgroup to a chunk: of a whole one all 16 loads are in flight before the first is used.  (Fewer workgroups that walk several chunks each are
+// slower: 351 us with 2048 of them against 323 for 65.1 M parameters.)  Last chunks first: the norm has just read their gradients.  Everything
+// else is read and written once and told so (nontemporal), so that the gradients stay in the cache from the norm to here: 403 -> 329 us.
 template <typename TG>
 __global__ void __launch_bounds__(256) adamw_f32_kernel(const AdamwChunk *__restrict__ table, const AdamwControl *__restrict__ ctl, AdamwArgs a,
                                                        unsigned *__restrict__ status) {
     if (!ctl->go) return;
-    const AdamwChunk c = table[blockIdx.x];
-    const float coef = ctl->coef, root2 = ctl->root2;
-    const float rate = mul_rn(ctl->rate, c.ls), fade = (float)(a.lr * (double)c.ls * (double)c.wd);
-    TG *gp = static_cast<TG *>(c.g);
-    float *mp = static_cast<float *>(c.m), *vp = static_cast<float *>(c.v);
+    const AdamwChunk c = table[gridDim.x - 1 - blockIdx.x];
+    const float rate = mul_rn(ctl->rate, c.ls), fade = (float)(a.lr * (double)c.ls * (double)c.wd), coef = ctl->coef, root2 = ctl->root2;
+    EMADAPT_GLOBAL TG *gp = global<TG>(c.g);
+    EMADAPT_GLOBAL float *wp = global<float>(c.w), *mp = global<float>(c.m), *vp = global<float>(c.v);
     bool bad = false;
-    for (int i = threadIdx.x * 4; i < c.n; i += 1024) {
-        float g[4], w[4], m[4], v[4], u;
-        if (i + 4 <= c.n) {
-            load4(gp + i, g); load4(c.w + i, w); load4(mp + i, m); load4(vp + i, v);
+    auto round4 = [&](int i, float (&g)[4], float (&w)[4], float (&m)[4], float (&v)[4]) {
 #pragma unroll
-            for (int k = 0; k < 4; k++) bad |= !adamw_element(g[k], m[k], v[k], u, w[k], coef, fade, rate, root2, a);
-            __builtin_memcpy(c.w + i, w, 16); __builtin_memcpy(mp + i, m, 16); __builtin_memcpy(vp + i, v, 16);
-            if (a.zero_grads) __builtin_memset(gp + i, 0, 4 * sizeof(TG));
-        } else {
-            for (int k = i; k < c.n; k++) {
-                float wk = c.w[k], mk = mp[k], vk = vp[k];
-                bad |= !adamw_element((float)gp[k], mk, vk, u, wk, coef, fade, rate, root2, a);
-                c.w[k] = wk; mp[k] = mk; vp[k] = vk;
-                if (a.zero_grads) gp[k] = (TG)0.f;
-            }
+        for (int k = 0; k < 4; k++) {
+            const Element e = adamw_element(g[k], m[k], v[k], w[k], coef, fade, rate, root2, a);
+            const bool ok = finite(e);   // (else the gradient took a moment out of the finite numbers: the element is left alone)
+            bad |= !ok;
+            m[k] = ok ? e.m : m[k];
+            v[k] = ok ? e.v : v[k];
+            w[k] = ok ? e.w : w[k];
+        }
+        store4_once(wp + i, w); store4_once(mp + i, m); store4_once(vp + i, v);
+        if (a.zero_grads) zero4(gp + i);
+    };
+    if (c.n == kChunk) {
+        float g[kRounds][4], w[kRounds][4], m[kRounds][4], v[kRounds][4];
+#pragma unroll
+        for (int q = 0; q < kRounds; q++) {
+            const int i = (q * 256 + threadIdx.x) * 4;
+            load4(gp + i, g[q]); load4_once(wp + i, w[q]); load4_once(mp + i, m[q]); load4_once(vp + i, v[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < kRounds; q++) round4((q * 256 + threadIdx.x) * 4, g[q], w[q], m[q], v[q]);
+    } else {
+        int i = threadIdx.x * 4;
+        for (; i + 4 <= c.n; i += 1024) {
+            float g[4], w[4], m[4], v[4];
+            load4(gp + i, g); load4_once(wp + i, w); load4_once(mp + i, m); load4_once(vp + i, v);
+            round4(i, g, w, m, v);
+        }
+        for (; i < c.n; i++) {   // (fewer than four, of one thread)
+            const Element e = adamw_element((float)gp[i], mp[i], vp[i], wp[i], coef, fade, rate, root2, a);
+            if (finite(e)) { wp[i] = e.w; mp[i] = e.m; vp[i] = e.v; }
+            else bad = true;
+            if (a.zero_grads) gp[i] = (TG)0.f;
         }
     }
     if (bad) status_raise(status, EMADAPT_STATUS_NAN_GRADIENT);
 }
 
 // ---- the 8-bit formats.  BITS mantissa bits; kShift = the lowest code bit's place in the fp32 pattern.
-template <int BITS> __device__ __forceinline__ int block_power(float top) {   // top >= 0, the block's largest magnitude
-    const unsigned e = (__float_as_uint(top) + (1u << (23 - BITS)) - 1u) >> 23;   // (past the largest code of its binade: one binade up)
+// largest pattern of a row of 16 lanes (patterns of numbers >= 0 are in their order), in all of them
+template <int CTRL> __device__ __forceinline__ unsigned dpp_max(unsigned x) {
+    const unsigned y = (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true);
+    return x > y ? x : y;
+}
+__device__ __forceinline__ unsigned row_top(float x) { return dpp_max<0x140>(dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(__float_as_uint(x))))); }
+template <int BITS> __device__ __forceinline__ int block_power(unsigned top) {   // pattern of the block's largest magnitude
+    const unsigned e = (top + (1u << (23 - BITS)) - 1u) >> 23;   // (past the largest code of its binade: one binade up)
     return (int)(e < 254u ? e : 254u);
 }
-template <int BITS> __device__ __forceinline__ unsigned code_of(float x, int e, unsigned draw) {   // x >= 0; draw < 2^(23 - BITS)
-    constexpr unsigned kTop = (16u << BITS) - 1u;
-    const unsigned c = (__float_as_uint(__builtin_amdgcn_ldexpf(x, 15 - e)) + draw) >> (23 - BITS);
-    return c < kTop ? c : kTop;
+// x >= 0 and at most the largest code of a block with this power; draw < 2^(23 - BITS): never above the largest code
+template <int BITS> __device__ __forceinline__ unsigned code_of(float x, int e, unsigned draw) {
+    return (__float_as_uint(__builtin_amdgcn_ldexpf(x, 15 - e)) + draw) >> (23 - BITS);
 }
 template <int BITS> __device__ __forceinline__ float value_of(unsigned code, int e) {
     return __builtin_amdgcn_ldexpf(__uint_as_float(code << (23 - BITS)), e - 15);
 }
-__device__ __forceinline__ float m_value(unsigned code, int e) {
-    const float x = value_of<3>(code & 0x7Fu, e);
-    return (code & 0x80u) ? -x : x;
+__device__ __forceinline__ float m_value(unsigned code, int e) {   // code: 8 bits
+    return __builtin_amdgcn_ldexpf(__uint_as_float((code << 24 & 0x80000000u) | (code & 0x7Fu) << 20), e - 15);
 }
 __device__ __forceinline__ unsigned m_code(float m, int e, unsigned draw) {
     return code_of<3>(fabsf(m), e, draw) | ((__float_as_uint(m) >> 24) & 0x80u);
 }
 __device__ __forceinline__ unsigned u_code(float u, int e, unsigned draw) {
-    const unsigned c = code_of<4>(u, e, draw);
-    return c == 0u && u > 0.f ? 1u : c;
+    const unsigned c = code_of<4>(u, e, draw), least = __float_as_uint(u) < 1u ? __float_as_uint(u) : 1u;
+    return c > least ? c : least;
 }
-// largest of a row of 16 lanes (a block of 64 elements, 4 to a lane), in all of them
-__device__ __forceinline__ float row_max(float x) {
-    for (int o = 8; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-    return x;
+// the formats' largest values at the uppermost power: what pack() is given is held to them (a step's moments are finite sums of what is there)
+constexpr float kMostM = 0x1.Ep127f, kMostU = 0x1.Fp127f;
+
+// One thread's four elements, 16 lanes to a block of 64: from the stored codes to the new ones.  n4: how many of them are the tensor's.
+struct Codes {
+    unsigned m, u, e;   // four codes each; the block's two powers
+};
+__device__ __forceinline__ bool adamw_codes(Codes &c, const float (&g)[4], float (&w)[4], int n4, unsigned long long unit, const DropKey key, float coef, float fade,
+                                            float rate, float root2, const AdamwArgs &a) {
+    float m[4], u[4], w1[4], mtop = 0.f, utop = 0.f, all = 0.f;
+    const int em = c.e & 0xFF, eu = c.e >> 8;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const float uk = value_of<4>(c.u >> (8 * k) & 0xFFu, eu);
+        const Element e = adamw_element(g[k], m_value(c.m >> (8 * k) & 0xFFu, em), mul_rn(uk, uk), w[k], coef, fade, rate, root2, a);
+        m[k] = e.m; u[k] = e.u; w1[k] = e.w;
+        all += fabsf(e.m) + e.v;
+    }
+    bool ok = true;
+    if (!(all < INFINITY)) {   // (a sum of finite ones may overflow too: looked at one by one)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float uk = value_of<4>(c.u >> (8 * k) & 0xFFu, eu), mk = m_value(c.m >> (8 * k) & 0xFFu, em);
+            if (!finite(adamw_element(g[k], mk, mul_rn(uk, uk), w[k], coef, fade, rate, root2, a))) {
+                m[k] = mk; u[k] = uk; w1[k] = w[k];
+                ok = false;
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if (k >= n4) m[k] = u[k] = 0.f;   // (past the tensor's end)
+        w[k] = w1[k];
+        mtop = fmaxf(mtop, fabsf(m[k]));
+        utop = fmaxf(utop, u[k]);
+    }
+    const int em1 = block_power<3>(row_top(mtop)), eu1 = block_power<4>(row_top(utop));
+    c.m = c.u = 0;
+    const unsigned line = drop_line(unit);   // (unit % 4 == 0: the four are behind one another)
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const unsigned h = drop_mix(key, line + (unsigned)k * kDropStep);
+        c.m |= m_code(m[k], em1, (h & 0xFFFFu) << 4) << (8 * k);
+        c.u |= u_code(u[k], eu1, (h >> 16) << 3) << (8 * k);
+    }
+    c.e = (unsigned)(em1 | eu1 << 8);
+    return ok;
 }
 
+// A workgroup to a round of a chunk, four elements to a thread: with the norm's and unpack()'s launches 262 us for 65.1 M parameters (f32 gradients)
+// against 281 where a workgroup has the chunk's four rounds in flight.  Some 85 vector-ALU slots to an element (generator 17, root 12, quotient
+// 7, both formats 25) are 140 us of the 190 that 65.1 M elements take, their 16.06 bytes 160: the two overlap.
 template <typename TG>
 __global__ void __launch_bounds__(256) adamw_u8_kernel(const AdamwChunk *__restrict__ table, const AdamwControl *__restrict__ ctl, AdamwArgs a,
                                                       unsigned *__restrict__ status) {
     if (!ctl->go) return;
-    const AdamwChunk c = table[blockIdx.x];
-    const float coef = ctl->coef, root2 = ctl->root2;
+    const unsigned at = gridDim.x - 1 - blockIdx.x;
+    const AdamwChunk c = table[at / kRounds];
+    const int i = (int)(at % kRounds) * 256 + threadIdx.x, n4 = c.n - i * 4;   // (n4: the thread's elements, may be more than 4)
+    if (n4 + (int)(threadIdx.x & 15) * 4 <= 0) return;                          // (whole rows of lanes: the codes' buffers reach that far)
     const float rate = mul_rn(ctl->rate, c.ls), fade = (float)(a.lr * (double)c.ls * (double)c.wd);
     const DropKey key = drop_key(((unsigned long long)a.seed << 32) + (unsigned)ctl->steps);
-    TG *gp = static_cast<TG *>(c.g);
-    unsigned char *mp = static_cast<unsigned char *>(c.m), *up = static_cast<unsigned char *>(c.v);
-    const int rounded = (c.n + kBlock - 1) / kBlock * kBlock;   // (whole rows of lanes: the codes' buffers reach that far)
-    bool bad = false;
-    for (int i = threadIdx.x * 4; i < rounded; i += 1024) {
-        float g[4] = {0.f, 0.f, 0.f, 0.f}, w[4] = {0.f, 0.f, 0.f, 0.f}, m[4], u[4];
-        if (i + 4 <= c.n) {
-            load4(gp + i, g); load4(c.w + i, w);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (i + k < c.n) { g[k] = (float)gp[i + k]; w[k] = c.w[i + k]; }
-        }
-        const unsigned mc = *reinterpret_cast<const unsigned *>(mp + i), uc = *reinterpret_cast<const unsigned *>(up + i);
-        const unsigned ee = *reinterpret_cast<const unsigned short *>(c.e + i / kBlock * 2);
-        const int em = ee & 0xFF, eu = ee >> 8;
-        float mtop = 0.f, utop = 0.f;
+    EMADAPT_GLOBAL TG *gp = global<TG>(c.g) + i * 4;
+    EMADAPT_GLOBAL float *wp = global<float>(c.w) + i * 4;
+    EMADAPT_GLOBAL unsigned *mp = global<unsigned>(c.m) + i, *up = global<unsigned>(c.v) + i;
+    EMADAPT_GLOBAL unsigned short *ep = global<unsigned short>(c.e) + i / 16;
+    float g[4], w[4];
+    Codes o;
+    o.m = __builtin_nontemporal_load(mp); o.u = __builtin_nontemporal_load(up); o.e = *ep;
+    if (n4 >= 4) {
+        load4(gp, g); load4_once(wp, w);
+    } else {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            m[k] = m_value(mc >> (8 * k) & 0xFFu, em);
-            u[k] = value_of<4>(uc >> (8 * k) & 0xFFu, eu);
-            float v = mul_rn(u[k], u[k]);
-            if (i + k < c.n) bad |= !adamw_element(g[k], m[k], v, u[k], w[k], coef, fade, rate, root2, a);
-            mtop = fmaxf(mtop, fabsf(m[k]));
-            utop = fmaxf(utop, u[k]);
-        }
-        const int em1 = block_power<3>(row_max(mtop)), eu1 = block_power<4>(row_max(utop));
-        unsigned mo = 0, uo = 0;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const unsigned h = drop_hash(key, c.unit + (unsigned)(i + k));
-            mo |= m_code(m[k], em1, (h & 0xFFFFu) << 4) << (8 * k);
-            uo |= u_code(u[k], eu1, (h >> 16) << 3) << (8 * k);
-        }
-        *reinterpret_cast<unsigned *>(mp + i) = mo;
-        *reinterpret_cast<unsigned *>(up + i) = uo;
-        if ((threadIdx.x & 15) == 0) *reinterpret_cast<unsigned short *>(c.e + i / kBlock * 2) = (unsigned short)(em1 | eu1 << 8);
-        if (i + 4 <= c.n) {
-            __builtin_memcpy(c.w + i, w, 16);
-            if (a.zero_grads) __builtin_memset(gp + i, 0, 4 * sizeof(TG));
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (i + k < c.n) { c.w[i + k] = w[k]; if (a.zero_grads) gp[i + k] = (TG)0.f; }
+            g[k] = k < n4 ? (float)gp[k] : 0.f;
+            w[k] = k < n4 ? wp[k] : 0.f;
         }
     }
-    if (bad) status_raise(status, EMADAPT_STATUS_NAN_GRADIENT);
+    const bool ok = adamw_codes(o, g, w, n4, c.unit + (unsigned)(i * 4), key, ctl->coef, fade, rate, ctl->root2, a);
+    __builtin_nontemporal_store(o.m, mp);
+    __builtin_nontemporal_store(o.u, up);
+    if ((threadIdx.x & 15) == 0) *ep = (unsigned short)o.e;
+    if (n4 >= 4) {
+        store4_once(wp, w);
+        if (a.zero_grads) zero4(gp);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (k < n4) { wp[k] = w[k]; if (a.zero_grads) gp[k] = (TG)0.f; }
+    }
+    if (!ok) status_raise(status, EMADAPT_STATUS_NAN_GRADIENT);
 }
 
 // codes <-> values, for checkpoints: four elements to a thread, rounding to nearest on the way in
@@ -277,10 +379,10 @@ __global__ void __launch_bounds__(256) adamw_pack_kernel(const float *__restrict
     // (n4 is a multiple of 16: a row of lanes is in the range as a whole or not at all)
     for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < n4; q += (long long)gridDim.x * 256) {
         float mv[4], uv[4], mtop = 0.f, utop = 0.f;
-        load4(m + q * 4, mv); load4(u + q * 4, uv);
+        load4((const EMADAPT_GLOBAL float *)m + q * 4, mv); load4((const EMADAPT_GLOBAL float *)u + q * 4, uv);
 #pragma unroll
-        for (int k = 0; k < 4; k++) { uv[k] = fmaxf(uv[k], 0.f); mtop = fmaxf(mtop, fabsf(mv[k])); utop = fmaxf(utop, uv[k]); }
-        const int em = block_power<3>(row_max(mtop)), eu = block_power<4>(row_max(utop));
+        for (int k = 0; k < 4; k++) { mv[k] = fminf(fmaxf(mv[k], -kMostM), kMostM); uv[k] = fminf(fmaxf(uv[k], 0.f), kMostU); mtop = fmaxf(mtop, fabsf(mv[k])); utop = fmaxf(utop, uv[k]); }
+        const int em = block_power<3>(row_top(mtop)), eu = block_power<4>(row_top(utop));
         unsigned mo = 0, uo = 0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -324,7 +426,7 @@ int emadapt_adamw_table(int count, const emadapt_adamw_tensor *tensors, int grad
     for (int k = 0; k < count; k++) {
         const emadapt_adamw_tensor &t = tensors[k];
         if (t.n == 0) continue;
-        if (!t.w || !t.g || !t.m || !t.v || !aligned(t.w, 4) || !aligned(t.g, gs) || t.unit < 0) return EMADAPT_ERR_INVALID;
+        if (!t.w || !t.g || !t.m || !t.v || !aligned(t.w, 4) || !aligned(t.g, gs) || t.unit < 0 || t.unit % 4) return EMADAPT_ERR_INVALID;
         // (codes are read four at a time and the powers of two by pairs; f32 moments at their own alignment)
         if (state == EMADAPT_ADAMW_U8 ? (!t.e || !aligned(t.m, 4) || !aligned(t.v, 4) || !aligned(t.e, 2)) : (!aligned(t.m, 4) || !aligned(t.v, 4)))
             return EMADAPT_ERR_INVALID;
@@ -349,24 +451,23 @@ int emadapt_adamw_table(int count, const emadapt_adamw_tensor *tensors, int grad
 int emadapt_adamw_step(const void *table, int64_t chunks, int grad_dtype, int state, void *control, size_t control_bytes, double lr, double beta1,
                        double beta2, double eps, float grad_scale, double max_norm, unsigned seed, int zero_grads, void *stream_) {
     if (!is_dt(grad_dtype) || (state != EMADAPT_ADAMW_F32 && state != EMADAPT_ADAMW_U8)) return EMADAPT_ERR_INVALID;
-    if (chunks < 0 || (chunks && !table) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 1e-30) || !(max_norm >= 0.0))
+    if (chunks < 0 || (chunks && !table) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 1e-16) || !(max_norm >= 0.0))
         return EMADAPT_ERR_INVALID;
     if (!control || control_bytes < sizeof(AdamwControl)) return EMADAPT_ERR_WORKSPACE;
-    if (chunks > 0x7FFFFFFF) return EMADAPT_ERR_UNSUPPORTED;
+    if (chunks > 0x7FFFFFFF / kRounds) return EMADAPT_ERR_UNSUPPORTED;
     hipStream_t stream = as_stream(stream_);
     const AdamwChunk *tab = static_cast<const AdamwChunk *>(table);
     AdamwControl *ctl = static_cast<AdamwControl *>(control);
     unsigned *status = status_word();
     const bool bf = grad_dtype == EMADAPT_DT_BF16;
     ProfScope prof(EMADAPT_K_OTHER, 0.0, (double)chunks * kChunk * ((bf ? 2.0 : 4.0) + 8.0 + (state == EMADAPT_ADAMW_U8 ? 4.06 : 16.0)), stream);
-    int nparts = 0;
+    const AdamwScalars sc = {lr, beta1, beta2, max_norm, grad_scale, max_norm > 0.0 ? 1 : 0, status_collective()};
     if (max_norm > 0.0) {
-        nparts = (int)(chunks < kParts ? (chunks ? chunks : 1) : kParts);
-        if (bf) hipLaunchKernelGGL(adamw_norm_kernel<__bf16>, dim3(nparts), dim3(256), 0, stream, tab, (long long)chunks, ctl);
-        else hipLaunchKernelGGL(adamw_norm_kernel<float>, dim3(nparts), dim3(256), 0, stream, tab, (long long)chunks, ctl);
-        if (int rc = launch_status()) return rc;
-    }
-    hipLaunchKernelGGL(adamw_control_kernel, dim3(1), dim3(256), 0, stream, ctl, nparts, lr, beta1, beta2, grad_scale, max_norm, status, status_collective());
+        const dim3 parts((unsigned)(chunks < 1 ? 1 : (chunks < kParts ? chunks : kParts)));
+        if (bf) hipLaunchKernelGGL(adamw_norm_kernel<__bf16>, parts, dim3(256), 0, stream, tab, (long long)chunks, ctl, sc, status);
+        else hipLaunchKernelGGL(adamw_norm_kernel<float>, parts, dim3(256), 0, stream, tab, (long long)chunks, ctl, sc, status);
+    } else
+        hipLaunchKernelGGL(adamw_control_kernel, dim3(1), dim3(1), 0, stream, ctl, sc, status);
     if (int rc = launch_status()) return rc;
     if (!chunks) return EMADAPT_OK;
     const AdamwArgs a = {(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, lr, seed, zero_grads};
@@ -375,8 +476,9 @@ int emadapt_adamw_step(const void *table, int64_t chunks, int grad_dtype, int st
         if (bf) hipLaunchKernelGGL(adamw_f32_kernel<__bf16>, grid, block, 0, stream, tab, ctl, a, status);
         else hipLaunchKernelGGL(adamw_f32_kernel<float>, grid, block, 0, stream, tab, ctl, a, status);
     } else {
-        if (bf) hipLaunchKernelGGL(adamw_u8_kernel<__bf16>, grid, block, 0, stream, tab, ctl, a, status);
-        else hipLaunchKernelGGL(adamw_u8_kernel<float>, grid, block, 0, stream, tab, ctl, a, status);
+        const dim3 rounds((unsigned)(chunks * kRounds));
+        if (bf) hipLaunchKernelGGL(adamw_u8_kernel<__bf16>, rounds, block, 0, stream, tab, ctl, a, status);
+        else hipLaunchKernelGGL(adamw_u8_kernel<float>, rounds, block, 0, stream, tab, ctl, a, status);
     }
     return launch_status();
 }

@@ -97,10 +97,14 @@ __device__ __forceinline__ DropKey drop_key(unsigned long long seed) {
     k.s2 = fmix32(k.s1 + 0x7F4A7C15u);
     return k;
 }
-__device__ __forceinline__ unsigned drop_hash(DropKey k, unsigned long long unit) {
-    unsigned h = (unsigned)unit * 0x9E3779B1u;
+constexpr unsigned kDropStep = 0x9E3779B1u;   // drop_line grows by this from a unit to the next
+__device__ __forceinline__ unsigned drop_line(unsigned long long unit) {
+    unsigned h = (unsigned)unit * kDropStep;
     const unsigned hi = (unsigned)(unit >> 32);
     if (__builtin_expect(hi != 0u, 0)) h += hi * 0x27D4EB2Fu;   // (tensors of 2^32 units and more: a branch the waves of a launch all skip)
+    return h;
+}
+__device__ __forceinline__ unsigned drop_mix(DropKey k, unsigned h) {
     h ^= k.s1;
     h ^= h >> 15;
     h *= 0x2C1B3C6Du;
@@ -110,7 +114,35 @@ __device__ __forceinline__ unsigned drop_hash(DropKey k, unsigned long long unit
     h ^= h >> 15;
     return h;
 }
+__device__ __forceinline__ unsigned drop_hash(DropKey k, unsigned long long unit) { return drop_mix(k, drop_line(unit)); }
 __device__ __forceinline__ unsigned drop_hash(unsigned long long seed, unsigned long long unit) { return drop_hash(drop_key(seed), unit); }
+
+// ---- reductions ----
+// Reductions over groups of L lanes, the result in all of them: DPP moves inside rows of 16 lanes, cross-row shuffles above.
+template <int CTRL> __device__ __forceinline__ float dpp(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false));
+}
+template <int L, typename F> __device__ __forceinline__ float group_reduce(float x, F op) {
+    if (L > 1) x = op(x, dpp<0xB1>(x));    // lanes 1 0 3 2
+    if (L > 2) x = op(x, dpp<0x4E>(x));    // lanes 2 3 0 1
+    if (L > 4) x = op(x, dpp<0x141>(x));   // the other quad of 8 lanes
+    if (L > 8) x = op(x, dpp<0x140>(x));   // the other half of 16 lanes
+    if (L > 16) x = op(x, __shfl_xor(x, 16));
+    if (L > 32) x = op(x, __shfl_xor(x, 32));
+    return x;
+}
+template <int L> __device__ __forceinline__ float group_max(float x) { return group_reduce<L>(x, [](float a, float b) { return fmaxf(a, b); }); }
+template <int L> __device__ __forceinline__ float group_sum(float x) { return group_reduce<L>(x, [](float a, float b) { return a + b; }); }
+// sum over the workgroup in 64 bits, in a fixed order; sh: a double per wave
+__device__ __forceinline__ double block_sum_f64(double v, double *sh) {
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double r = 0.0;
+    for (int k = 0; k < (int)(blockDim.x >> 6); k++) r += sh[k];
+    __syncthreads();
+    return r;
+}
 
 // ---- per-kernel event timing (bench.py roofline; see emadapt_prof_* in emadapt.h) ----
 struct ProfScope {

@@ -75,21 +75,6 @@ template <typename T> __device__ __forceinline__ void grad_vec(Raw r, float base
     }
 }
 
-// Reductions over groups of L lanes, the result in all of them: DPP moves inside rows of 16 lanes, cross-row shuffles above.
-template <int CTRL> __device__ __forceinline__ float dpp(float x) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false));
-}
-template <int L, typename F> __device__ __forceinline__ float group_reduce(float x, F op) {
-    if (L > 1) x = op(x, dpp<0xB1>(x));    // lanes 1 0 3 2
-    if (L > 2) x = op(x, dpp<0x4E>(x));    // lanes 2 3 0 1
-    if (L > 4) x = op(x, dpp<0x141>(x));   // the other quad of 8 lanes
-    if (L > 8) x = op(x, dpp<0x140>(x));   // the other half of 16 lanes
-    if (L > 16) x = op(x, __shfl_xor(x, 16));
-    if (L > 32) x = op(x, __shfl_xor(x, 32));
-    return x;
-}
-template <int L> __device__ __forceinline__ float group_max(float x) { return group_reduce<L>(x, [](float a, float b) { return fmaxf(a, b); }); }
-template <int L> __device__ __forceinline__ float group_sum(float x) { return group_reduce<L>(x, [](float a, float b) { return a + b; }); }
 __device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.f : m; }
 
 // running maximum and sum of exponentials of a part of a row
@@ -106,16 +91,6 @@ template <int W> __device__ __forceinline__ MaxSum block_join(MaxSum wave, MaxSu
     r.s = group_sum<W>(t.s * __expf(t.m - finite_or_0(r.m)));
     return r;
 }
-__device__ __forceinline__ double block_sum_f64(double v, double *sh) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double r = 0.0;
-    for (int k = 0; k < (int)(blockDim.x >> 6); k++) r += sh[k];
-    __syncthreads();
-    return r;
-}
-
 struct Rows {
     const void *logits;
     const long long *labels;

@@ -1004,8 +1004,8 @@ class AdamW:
             raise ValueError("state must be 'f32' or 'u8', got %r" % (state,))
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
             raise ValueError("betas must be in [0, 1), got %r" % (betas,))
-        if not eps >= 1e-30:
-            raise ValueError("eps must be at least 1e-30, got %r" % (eps,))
+        if not eps >= 1e-16:
+            raise ValueError("eps must be at least 1e-16, got %r" % (eps,))
         for k, p in enumerate(params):
             _check(p, name="params[%d]" % k)
             if p.device != params[0].device:

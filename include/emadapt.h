@@ -603,7 +603,7 @@ int emadapt_preference_loss(const void *logits, int dtype, int64_t ldl, const in
  * replayed; two steps on one control block belong on one stream.
  * A raised status word makes the step a no-op (not in collective mode: the gradient carries the failure).  A norm that is not finite
  * makes the step a no-op; an element whose moments would leave the finite numbers is left alone; both raise EMADAPT_STATUS_NAN_GRADIENT.
- * zero_grads: the gradients are zeroed behind the step (the clean op of deeplab.py:204).  beta1, beta2 in [0, 1), eps >= 1e-30. */
+ * zero_grads: the gradients are zeroed behind the step (the clean op of deeplab.py:204).  beta1, beta2 in [0, 1), eps >= 1e-16. */
 #define EMADAPT_ADAMW_F32 0
 #define EMADAPT_ADAMW_U8 1
 typedef struct emadapt_adamw_tensor {
@@ -612,7 +612,7 @@ typedef struct emadapt_adamw_tensor {
     void *m, *v;
     void *e;             /* EMADAPT_ADAMW_U8 only */
     int64_t n;
-    int64_t unit;        /* first element's place in the generator's sequence (e.g. its offset in the state buffers) */
+    int64_t unit;        /* first element's place in the generator's sequence, a multiple of 4 (e.g. its offset in the state buffers) */
     float weight_decay, lr_scale;
 } emadapt_adamw_tensor;
 int64_t emadapt_adamw_chunks(int count, const emadapt_adamw_tensor *tensors);
