@@ -28,20 +28,22 @@ template <> __device__ __forceinline__ void unpack<__bf16>(Raw r, float (&v)[8])
         v[2 * k + 1] = __uint_as_float(r[k] & 0xFFFF0000u);
     }
 }
+typedef unsigned U4 __attribute__((ext_vector_type(4), aligned(2), may_alias));
+typedef unsigned U2 __attribute__((ext_vector_type(2), aligned(2), may_alias));
+// ONCE: read for the last time (nontemporal: what is in the cache stays there)
+template <bool ONCE, typename T> __device__ __forceinline__ Raw load16(const T *p) {
+    return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const U4 *>(p)) : *reinterpret_cast<const U4 *>(p);
+}
 template <typename T> __device__ __forceinline__ Raw pack_raw(const T (&t)[Vec<T>::N]) {
     Raw r;
     __builtin_memcpy(&r, t, 16);
     return r;
 }
 // Vector at element i of a row of C elements (ldl with the padding); what is not one of the C is -inf: no weight in any sum of exponentials.
-template <typename T> __device__ __forceinline__ Raw load_row(const T *z, int i, int C, int ldl) {
+template <bool ONCE, typename T> __device__ __forceinline__ Raw load_row(const T *z, int i, int C, int ldl) {
     constexpr int N = Vec<T>::N;
     T t[N];
-    if (i + N <= C) {
-        Raw r;
-        __builtin_memcpy(&r, z + i, 16);
-        return r;
-    }
+    if (i + N <= C) return load16<ONCE>(z + i);
     if (i + N <= ldl) {
         __builtin_memcpy(t, z + i, 16);
 #pragma unroll
@@ -52,12 +54,30 @@ template <typename T> __device__ __forceinline__ Raw load_row(const T *z, int i,
     }
     return pack_raw<T>(t);
 }
-template <typename T, int N> __device__ __forceinline__ void store_row(T *d, int i, int ldl, const float (&v)[N]) {
+// (the empty asm keeps the compiler from making one plain store of the two)
+template <typename U> __device__ __forceinline__ void put(char *p, const char *t, bool once) {
+    U r;
+    __builtin_memcpy(&r, t, sizeof(r));
+    if (once) {
+        asm volatile("");
+        __builtin_nontemporal_store(r, reinterpret_cast<U *>(p));
+        asm volatile("");
+    } else
+        *reinterpret_cast<U *>(p) = r;
+}
+template <typename T, int N> __device__ __forceinline__ void store_row(T *d, int i, int ldl, const float (&v)[N], bool once) {
     T t[N];
 #pragma unroll
     for (int k = 0; k < N; k++) t[k] = (T)v[k];
-    if (i + N <= ldl) __builtin_memcpy(d + i, t, sizeof(t));
-    else {
+    char *p = reinterpret_cast<char *>(d + i);
+    const char *q = reinterpret_cast<const char *>(t);
+    if (i + N <= ldl) {
+        if constexpr (sizeof(t) == 8) put<U2>(p, q, once);
+        else {
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(t); k += 16) put<U4>(p + k, q + k, once);
+        }
+    } else {
 #pragma unroll
         for (int k = 0; k < N; k++)
             if (i + k < ldl) d[i + k] = t[k];
@@ -81,6 +101,8 @@ __device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 
 struct MaxSum {
     float m, s;
 };
+// the label's log-probability in a row with this maximum and sum (64 bits: the differences are exact, the sum's logarithm is what is rounded)
+__device__ __forceinline__ double logp_of(float z, MaxSum row) { return ((double)z - (double)row.m) - (double)logf(row.s); }
 // over a workgroup of W waves, from each wave's pair: one barrier, sh is free again at the next one
 template <int W> __device__ __forceinline__ MaxSum block_join(MaxSum wave, MaxSum *sh) {
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = wave;
@@ -96,10 +118,14 @@ struct Rows {
     const long long *labels;
     long long ldl, M;
     int C;
+    bool once;   // the gradient is too large to stay in the cache: it is not left there
 };
 
 // dz = [c = label] coef - exp(z - base) coef / sum (base, sum: the row's maximum and sum; without sum the log-sum-exp): every thread its vectors of the flattened [M][vectors per row], kUnroll of them in flight.  A
 // workgroup's vectors lie behind one another; their rows come from one 64-bit division for the workgroup and a 32-bit one for each vector.
+#ifndef GONCE
+#define GONCE true
+#endif
 constexpr int kUnroll = 4;
 template <typename T, typename TD>
 __global__ void __launch_bounds__(256) row_grad_kernel(Rows a, const float *__restrict__ base, const float *__restrict__ sum, const float *__restrict__ coef, TD *__restrict__ dlogits,
@@ -118,7 +144,7 @@ __global__ void __launch_bounds__(256) row_grad_kernel(Rows a, const float *__re
         row[q] = b + q * 256 + threadIdx.x < total ? r0 + dr : -1;
         if (row[q] < 0) continue;
         at[q] = (int)(o - dr * nvec) * N;
-        raw[q] = load_row(static_cast<const T *>(a.logits) + row[q] * a.ldl, at[q], a.C, (int)a.ldl);
+        raw[q] = load_row<GONCE>(static_cast<const T *>(a.logits) + row[q] * a.ldl, at[q], a.C, (int)a.ldl);
         const long long lab = a.labels[row[q]];
         const bool used = lab >= 0 && lab < a.C;
         hit[q] = used ? (int)lab : -(1 << 30);
@@ -135,7 +161,7 @@ __global__ void __launch_bounds__(256) row_grad_kernel(Rows a, const float *__re
 #pragma unroll
             for (int k = 0; k < N; k++) v[k] = 0.f;
         }
-        store_row<TD>(dlogits + row[q] * a.ldl, at[q], (int)a.ldl, v);
+        store_row<TD>(dlogits + row[q] * a.ldl, at[q], (int)a.ldl, v, a.once);
     }
 }
 
@@ -146,7 +172,7 @@ struct Policy {
     const float *old_logp, *ref_logp, *adv, *weight;
     double low, high;   // the ratio's borders, 1 - clip_low and 1 + clip_high
     double log_low, log_high;
-    float kl, scale;
+    float kl, scale, tol;
 };
 struct PolicyTerms {
     double loss, surrogate, kl, clipped;
@@ -179,11 +205,13 @@ __device__ __forceinline__ float policy_row(float log_ratio, float q, bool has_r
 __device__ __forceinline__ bool past_border(double log_ratio, float adv, const Policy &p) {
     return adv > 0.f ? log_ratio > p.log_high : (adv < 0.f ? log_ratio < p.log_low : false);
 }
-// f32's log ratio is off by less than this: rounding of the sum over a row (at most 2^-15 of it), of exponents and of the differences
-__device__ __forceinline__ bool near_border(float log_ratio, float magnitude, float adv, const Policy &p) {
-    const float tol = 1e-4f + 4.8e-7f * magnitude;
-    const float border = adv > 0.f ? (float)p.log_high : (float)p.log_low;
-    return adv != 0.f && fabsf(log_ratio - border) < tol;
+// The log ratio from an f32 sum of exponentials (z, maximum and old_logp are taken in 64 bits) is off by less than tol: with h = 2^-24, 3 h for each
+// of the `steps` additions and rescalings behind one another and 30 h for the trees, 2 h |z - m| + 2 h for an exponential -- whose mean over the
+// softmax is at most log C --, and 2 h log C for the logarithm; half as much again.
+__host__ __device__ inline float border_tol(int steps, int C) { return 1.5f * 0x1p-24f * (3.f * steps + 40.f + 5.f * logf((float)C)); }
+__device__ __forceinline__ bool near_border(double log_ratio, float adv, const Policy &p) {
+    const double border = adv > 0.f ? p.log_high : p.log_low;
+    return adv != 0.f && fabs(log_ratio - border) < (double)p.tol;
 }
 // sum over elements `first`, first + step, .. of the row of exp(z - z_label) in 64 bits
 template <typename T>
@@ -203,25 +231,30 @@ struct Outputs {
     float *logp, *lse;          // kLogp: any of these may be null
     float *base, *sum, *zero;   // kLogp: the rows' maximum and sum of exponentials; a value per row set to 0
     void *dlogits;
-    double *partial;            // [gridDim.x][4]
+    double *partial;            // a workgroup's sums, [gridDim.x][4]
+    unsigned char *near;        // rows to be looked at in 64 bits (policy_finish_kernel)
+    unsigned *ticket;           // its ticket, to be zeroed
+    MaxSum *parts;              // [M][gridDim.y] of rows in several parts
 };
 
-// A row's part of the policy loss once its log-sum-exp is known.  The ratio is cut where exact arithmetic on the inputs cuts it: for a row near
-// a border `exact` gives logp in 64 bits.  The sums are taken by one thread of the row's (count).
-template <typename E>
-__device__ __forceinline__ float policy_of_row(const Policy &p, long long r, float z, MaxSum row, bool count, E exact, float &lp, PolicyTerms &t) {
-    const float oldp = p.old_logp[r], adv = p.adv[r], w = p.weight ? p.weight[r] : 1.f, refp = p.ref_logp ? p.ref_logp[r] : 0.f;
-    const float log_sum = logf(row.s);
-    lp = (z - row.m) - log_sum;
-    float lr = lp - oldp;
-    bool clipped = past_border(lr, adv, p);
-    if (near_border(lr, fabsf(z - row.m) + log_sum + fabsf(oldp), adv, p)) {
-        const double lp64 = exact();
-        lp = (float)lp64;
-        lr = (float)(lp64 - (double)oldp);
-        clipped = past_border(lp64 - (double)oldp, adv, p);
-    }
-    return policy_row(lr, refp - lp, p.ref_logp != nullptr, adv, w, p, clipped, count, t);
+// A row's part of the policy loss once its log-sum-exp is known, as f32 sees it; near: exact arithmetic may cut the ratio where f32 does not.
+struct PolicyInputs {
+    float oldp, adv, w, refp;
+    bool has_ref;
+};
+__device__ __forceinline__ PolicyInputs policy_inputs(const Policy &p, long long r) {
+    return {p.old_logp[r], p.adv[r], p.weight ? p.weight[r] : 1.f, p.ref_logp ? p.ref_logp[r] : 0.f, p.ref_logp != nullptr};
+}
+__device__ __forceinline__ float policy_of_row(const Policy &p, const PolicyInputs &x, float z, MaxSum row, bool count, float &lp, bool &near, PolicyTerms &t) {
+    const double lp64 = logp_of(z, row), lr = lp64 - (double)x.oldp;
+    lp = (float)lp64;
+    near = near_border(lr, x.adv, p);
+    return policy_row((float)lr, (float)((double)x.refp - lp64), x.has_ref, x.adv, x.w, p, past_border(lr, x.adv, p), count && !near, t);
+}
+__device__ __forceinline__ float policy_of_exact(const Policy &p, const PolicyInputs &x, double lp64, bool count, float &lp, PolicyTerms &t) {
+    const double lr = lp64 - (double)x.oldp;
+    lp = (float)lp64;
+    return policy_row((float)lr, (float)((double)x.refp - lp64), x.has_ref, x.adv, x.w, p, past_border(lr, x.adv, p), count, t);
 }
 
 // L lanes to a row, a vector of the padded row to a lane.
@@ -238,7 +271,7 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
         bool used = lab >= 0 && lab < a.C;
         if (MODE != kLogp && p.weight) used = used && p.weight[r] != 0.f;
         const int i = lane * N;
-        const Raw raw = load_row(z, i, a.C, (int)a.ldl);
+        const Raw raw = load_row<MODE != kLogp>(z, i, a.C, (int)a.ldl);
         float v[N], m = -INFINITY, s = 0.f;
         unpack<T>(raw, v);
 #pragma unroll
@@ -251,13 +284,17 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
         float lp = 0.f, f = 0.f;
         if (used) {
             const float zl = (float)z[lab];
-            if (MODE == kLogp) lp = (zl - m) - logf(s);
-            else
-                f = policy_of_row(p, r, zl, MaxSum{m, s}, lane == 0, [&] {
+            if (MODE == kLogp) lp = (float)logp_of(zl, MaxSum{m, s});
+            else {
+                const PolicyInputs x = policy_inputs(p, r);
+                bool near;
+                f = policy_of_row(p, x, zl, MaxSum{m, s}, lane == 0, lp, near, t);
+                if (near) {
                     double e = exact_part(z, a.C, lab, lane, L);
                     for (int o = L / 2; o > 0; o >>= 1) e += __shfl_xor(e, o);
-                    return -log(e);
-                }, lp, t);
+                    f = policy_of_exact(p, x, -log(e), lane == 0, lp, t);
+                }
+            }
         }
         if (lane == 0) {
             if (MODE != kLogp || out.logp) out.logp[r] = lp;
@@ -273,7 +310,7 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
 #pragma unroll
                 for (int e = 0; e < N; e++) v[e] = 0.f;
             }
-            store_row<TD>(static_cast<TD *>(out.dlogits) + r * a.ldl, i, (int)a.ldl, v);
+            store_row<TD>(static_cast<TD *>(out.dlogits) + r * a.ldl, i, (int)a.ldl, v, a.once);
         }
     }
     if (MODE != kLogp) {
@@ -292,38 +329,49 @@ template <int N> __device__ __forceinline__ void take(const float (&v)[N], float
 #pragma unroll
     for (int e = 0; e < N; e++) top = fmaxf(top, v[e]);
     const float m0 = finite_or_0(top);
-    s *= __expf(m - m0);
+    float x[N];
 #pragma unroll
-    for (int e = 0; e < N; e++) s += __expf(v[e] - m0);
+    for (int e = 0; e < N; e++) x[e] = __expf(v[e] - m0);
+#pragma unroll
+    for (int w = N / 2; w > 0; w /= 2)   // (a tree: the rounding of the sum, and with it near_border's width, goes by the vectors)
+#pragma unroll
+        for (int e = 0; e < w; e++) x[e] += x[e + w];
+    s = __builtin_fmaf(s, __expf(m - m0), x[0]);
     m = top;
 }
 
 // A workgroup of W waves to a row, NV whole vectors to a thread, and the C % N last elements one to a thread.
 template <typename T, typename TD, int W, int NV, int MODE>
-__global__ void __launch_bounds__(64 * W) block_kernel(Rows a, Policy p, Outputs out) {
+__global__ void __launch_bounds__(64 * W, 4) block_kernel(Rows a, Policy p, Outputs out) {
     constexpr int N = Vec<T>::N, kThreads = 64 * W;
     __shared__ MaxSum pair[2][W];
-    __shared__ double sh[W];
     __shared__ PolicyTerms terms;   // (thread 0's: registers are short here)
-    if (threadIdx.x == 0) terms = {0, 0, 0, 0};
-    const int nfull = a.C / N, last = nfull * N + threadIdx.x;
+    if (threadIdx.x == 0) {
+        terms = {0, 0, 0, 0};
+        if (blockIdx.x == 0) *out.ticket = 0u;
+    }
+    const int nfull = a.C / N;
     int turn = 0;
     for (long long r = blockIdx.x; r < a.M; r += gridDim.x, turn ^= 1) {
         const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
+        unsigned tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));   // (or the row loop's registers go to the addresses and comparisons of all NV vectors, made once in front of it)
+        const int last = nfull * N + (int)tid;
         const long long lab = a.labels[r];
-        bool used = lab >= 0 && lab < a.C;
-        if (p.weight) used = used && p.weight[r] != 0.f;
+        const PolicyInputs x = policy_inputs(p, r);   // (in front of the row: their way to memory is the row's)
+        const bool used = lab >= 0 && lab < a.C && x.w != 0.f;
+        const float zl = (float)z[used ? lab : 0];
         Raw raw[NV];
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int i = threadIdx.x + k * kThreads;
-            if (i < nfull) __builtin_memcpy(&raw[k], z + i * N, 16);
+        for (int k = 0; k < NV; k++) {   // (all of them load, the ones past the row its last vector: the waits below can then count the loads)
+            const int i = (int)tid + k * kThreads, j = i < nfull ? i : nfull - 1;
+            raw[k] = load16<true>(reinterpret_cast<const T *>(reinterpret_cast<const char *>(z) + (unsigned)j * 16u));
         }
         float m = last < a.C ? (float)z[last] : -INFINITY;
         float s = last < a.C ? __expf(m - finite_or_0(m)) : 0.f;
 #pragma unroll
         for (int k = 0; k < NV; k++)
-            if ((int)threadIdx.x + k * kThreads < nfull) {
+            if ((int)tid + k * kThreads < nfull) {
                 float v[N];
                 unpack<T>(raw[k], v);
                 take(v, m, s);
@@ -334,14 +382,15 @@ __global__ void __launch_bounds__(64 * W) block_kernel(Rows a, Policy p, Outputs
         s = group_sum<64>(s * __expf(m - finite_or_0(mw)));
         const MaxSum row = block_join<W>(MaxSum{mw, s}, pair[turn]);   // (two buffers: a wave may be a row ahead)
         float lp = 0.f, f = 0.f;
-        if (used) {   // (the same in every thread: the barriers inside are met by all)
+        bool near = false;
+        if (used) {
             PolicyTerms one = {0, 0, 0, 0};
-            f = policy_of_row(p, r, (float)z[lab], row, threadIdx.x == 0, [&] { return -log(block_sum_f64(exact_part(z, a.C, lab, threadIdx.x, kThreads), sh)); }, lp, one);
+            f = policy_of_row(p, x, zl, row, threadIdx.x == 0, lp, near, one);
             if (threadIdx.x == 0) {
                 terms.loss += one.loss; terms.surrogate += one.surrogate; terms.kl += one.kl; terms.clipped += one.clipped;
             }
         }
-        if (threadIdx.x == 0) out.logp[r] = lp;
+        if (threadIdx.x == 0) { out.logp[r] = lp; out.near[r] = near; }
         TD *d = static_cast<TD *>(out.dlogits) + r * a.ldl;
         const int hit = used ? (int)lab : -(1 << 30);
         const float fs = f * __builtin_amdgcn_rcpf(row.s);
@@ -349,19 +398,20 @@ __global__ void __launch_bounds__(64 * W) block_kernel(Rows a, Policy p, Outputs
             d[i] = (TD)(f != 0.f && i < a.C ? (i == hit ? f : 0.f) - __expf((float)z[i] - row.m) * fs : 0.f);
         if (f == 0.f) {   // (a row that takes no part)
 #pragma unroll 1
-            for (int i = threadIdx.x; i < nfull; i += kThreads) {
+            for (int i = tid; i < nfull; i += kThreads) {
                 const float v[N] = {};
-                store_row<TD>(d, i * N, nfull * N, v);
+                store_row<TD>(d, i * N, nfull * N, v, a.once);
             }
             continue;
         }
+        asm volatile("" : "+v"(tid));
 #pragma unroll
         for (int k = 0; k < NV; k++) {
-            const int i = threadIdx.x + k * kThreads;
+            const int i = (int)tid + k * kThreads;
             if (i < nfull) {
                 float v[N];
                 grad_vec<T>(raw[k], row.m, fs, f, hit - i * N, v);
-                store_row<TD>(d, i * N, nfull * N, v);
+                store_row<TD>(reinterpret_cast<TD *>(reinterpret_cast<char *>(d) + (unsigned)i * (unsigned)(N * sizeof(TD))), 0, N, v, a.once);
             }
         }
     }
@@ -372,7 +422,7 @@ __global__ void __launch_bounds__(64 * W) block_kernel(Rows a, Policy p, Outputs
 }
 
 // One workgroup to a row of any length, read once: a running maximum and sum for every thread, kAhead vectors in flight.
-template <typename T, int W>
+template <typename T, int W, bool ONCE>
 __global__ void __launch_bounds__(64 * W) stream_stats_kernel(Rows a, Outputs out) {
     constexpr int N = Vec<T>::N, kThreads = 64 * W, kAhead = 4;
     __shared__ MaxSum pair[2][W];
@@ -381,10 +431,14 @@ __global__ void __launch_bounds__(64 * W) stream_stats_kernel(Rows a, Outputs ou
         const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
         const long long lab = a.labels[r];
         float m = -INFINITY, s = 0.f;
-        for (int i0 = threadIdx.x * N; i0 < a.C; i0 += kThreads * N * kAhead) {
+        // (part y of the row: whole vectors, the last part with the rest)
+        const int per = ((a.C + (int)gridDim.y * N - 1) / ((int)gridDim.y * N)) * N, begin = per * (int)blockIdx.y;
+        const int end = begin + per < a.C ? begin + per : a.C;
+        int i0 = begin + threadIdx.x * N;
+        for (; i0 + (kAhead - 1) * kThreads * N + N <= end; i0 += kThreads * N * kAhead) {
             Raw raw[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; k++) raw[k] = load_row(z, i0 + k * kThreads * N, a.C, (int)a.ldl);
+            for (int k = 0; k < kAhead; k++) raw[k] = load16<ONCE>(z + i0 + k * kThreads * N);
 #pragma unroll
             for (int k = 0; k < kAhead; k++) {
                 float v[N];
@@ -392,22 +446,31 @@ __global__ void __launch_bounds__(64 * W) stream_stats_kernel(Rows a, Outputs ou
                 take(v, m, s);
             }
         }
+        for (; i0 < end; i0 += kThreads * N) {
+            float v[N];
+            unpack<T>(load_row<ONCE>(z, i0, end, end), v);
+            take(v, m, s);
+        }
         const float mw = group_max<64>(m);
         s = group_sum<64>(s * __expf(m - finite_or_0(mw)));
         const MaxSum row = block_join<W>(MaxSum{mw, s}, pair[turn]);
-        if (threadIdx.x == 0) {
-            const float log_sum = logf(row.s);
-            if (out.lse) out.lse[r] = row.m + log_sum;
+        if (threadIdx.x != 0) continue;
+        if (out.parts) out.parts[r * gridDim.y + blockIdx.y] = row;
+        else {
+            if (out.lse) out.lse[r] = row.m + logf(row.s);
             if (out.base) { out.base[r] = row.m; out.sum[r] = row.s; }
-            if (out.logp) out.logp[r] = lab >= 0 && lab < a.C ? ((float)z[lab] - row.m) - log_sum : 0.f;
+            if (out.logp) out.logp[r] = lab >= 0 && lab < a.C ? (float)logp_of((float)z[lab], row) : 0.f;
             if (out.zero) out.zero[r] = 0.f;
         }
     }
 }
 
+// The rows' terms where the log-sum-exp comes from a launch of its own, as the rows' maximum and sum or in `splits` parts of each row.  One
+// workgroup also writes the sums.
 template <typename T>
-__global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const float *__restrict__ base, const float *__restrict__ sum, float *__restrict__ logp, float *__restrict__ coef,
-                                                        double *__restrict__ partial) {
+__global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const MaxSum *__restrict__ parts, int splits, float *__restrict__ base,
+                                                        float *__restrict__ sum, float *__restrict__ logp, float *__restrict__ coef,
+                                                        double *__restrict__ partial, float *__restrict__ sums) {
     __shared__ double sh[4];
     __shared__ unsigned long long mask[4];
     PolicyTerms t = {0, 0, 0, 0};
@@ -417,14 +480,19 @@ __global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const
         if (r < a.M) {
             const long long lab = a.labels[r];
             const float w = p.weight ? p.weight[r] : 1.f;
+            MaxSum row;
+            if (parts) {
+                row = parts[r * splits];
+                for (int k = 1; k < splits; k++) row.m = fmaxf(row.m, parts[r * splits + k].m);
+                row.s = 0.f;
+                for (int k = 0; k < splits; k++) row.s += parts[r * splits + k].s * __expf(parts[r * splits + k].m - finite_or_0(row.m));
+                base[r] = row.m;
+                sum[r] = row.s;
+            } else
+                row = {base[r], sum[r]};
             float lp = 0.f, f = 0.f;
-            if (lab >= 0 && lab < a.C && w != 0.f) {
-                const float z = (float)(static_cast<const T *>(a.logits) + r * a.ldl)[lab], m = base[r], log_sum = logf(sum[r]), oldp = p.old_logp[r], adv = p.adv[r];
-                lp = (z - m) - log_sum;
-                const float lr = lp - oldp;
-                again = near_border(lr, fabsf(z - m) + log_sum + fabsf(oldp), adv, p);
-                if (!again) f = policy_row(lr, p.ref_logp ? p.ref_logp[r] - lp : 0.f, p.ref_logp != nullptr, adv, w, p, past_border(lr, adv, p), true, t);
-            }
+            if (lab >= 0 && lab < a.C && w != 0.f)
+                f = policy_of_row(p, policy_inputs(p, r), (float)(static_cast<const T *>(a.logits) + r * a.ldl)[lab], row, true, lp, again, t);
             logp[r] = lp;
             coef[r] = f;
         }
@@ -435,14 +503,11 @@ __global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const
         for (int q = 0; q < 4; q++)
             for (unsigned long long left = mask[q]; left; left &= left - 1) {
                 const long long rr = r0 + q * 64 + (__ffsll((long long)left) - 1);
-                const long long lab = a.labels[rr];
-                const double lp = -log(block_sum_f64(exact_part(static_cast<const T *>(a.logits) + rr * a.ldl, a.C, lab, threadIdx.x, 256), sh));
+                const double lp64 = -log(block_sum_f64(exact_part(static_cast<const T *>(a.logits) + rr * a.ldl, a.C, a.labels[rr], threadIdx.x, 256), sh));
                 if (threadIdx.x == 0) {
-                    const float adv = p.adv[rr], lpf = (float)lp;
-                    const double lr = lp - (double)p.old_logp[rr];
-                    logp[rr] = lpf;
-                    coef[rr] = policy_row((float)lr, p.ref_logp ? p.ref_logp[rr] - lpf : 0.f, p.ref_logp != nullptr, adv, p.weight ? p.weight[rr] : 1.f, p,
-                                          past_border(lr, adv, p), true, t);
+                    float lp;
+                    coef[rr] = policy_of_exact(p, policy_inputs(p, rr), lp64, true, lp, t);
+                    logp[rr] = lp;
                 }
             }
         __syncthreads();
@@ -450,17 +515,66 @@ __global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const
     const double s[4] = {t.loss, t.surrogate, t.kl, t.clipped};
     for (int k = 0; k < 4; k++) {
         const double v = block_sum_f64(s[k], sh);
-        if (threadIdx.x == 0) partial[(long long)blockIdx.x * 4 + k] = v;
+        if (threadIdx.x == 0) {
+            if (gridDim.x == 1) sums[k] = (float)v;
+            else partial[(long long)blockIdx.x * 4 + k] = v;
+        }
     }
 }
 
-__global__ void __launch_bounds__(256) policy_sums_kernel(const double *__restrict__ partial, int n, float *__restrict__ sums) {
-    __shared__ double sh[4];
-    for (int k = 0; k < 4; k++) {
-        double s = 0.0;
-        for (int i = threadIdx.x; i < n; i += 256) s += partial[(long long)i * 4 + k];
-        s = block_sum_f64(s, sh);
-        if (threadIdx.x == 0) sums[k] = (float)s;
+// The sums of the launch before, and its rows near a border (near, or null) in 64 bits: 1024 rows to a workgroup, nearly all of which find none.
+// Their terms were left out there; logp and the gradient are written again.  The last workgroup adds everything up in a fixed order.
+template <typename T, typename TD>
+__global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, Outputs out, int nparts, double *__restrict__ fixed, float *__restrict__ sums) {
+    __shared__ double sh[16][4];
+    __shared__ double one[16];
+    __shared__ unsigned long long mask[16];
+    __shared__ bool last;
+    PolicyTerms t = {0, 0, 0, 0};
+    if (out.near) {
+        const long long r0 = (long long)blockIdx.x * 1024, mine = r0 + threadIdx.x;
+        const unsigned long long b = __ballot(mine < a.M && out.near[mine]);
+        if ((threadIdx.x & 63) == 0) mask[threadIdx.x >> 6] = b;
+        __syncthreads();
+        for (int q = 0; q < 16; q++)
+            for (unsigned long long left = mask[q]; left; left &= left - 1) {
+                const long long r = r0 + q * 64 + (__ffsll((long long)left) - 1), lab = a.labels[r];
+                const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
+                const double lp64 = -log(block_sum_f64(exact_part(z, a.C, lab, threadIdx.x, 1024), one));
+                float lp;
+                const float f = policy_of_exact(p, policy_inputs(p, r), lp64, threadIdx.x == 0, lp, t);
+                if (threadIdx.x == 0) out.logp[r] = lp;
+                if (!out.dlogits) continue;
+                const float lse = (float)((double)(float)z[lab] - lp64);
+                TD *d = static_cast<TD *>(out.dlogits) + r * a.ldl;
+#pragma unroll 1
+                for (int i = threadIdx.x; i < a.C; i += 1024) d[i] = (TD)(f == 0.f ? 0.f : (i == (int)lab ? f : 0.f) - __expf((float)z[i] - lse) * f);
+            }
+        // (a ticket among few workgroups; the part is where every CU sees it before the ticket counts it)
+        if (threadIdx.x == 0) {
+            const double s[4] = {t.loss, t.surrogate, t.kl, t.clipped};
+            for (int k = 0; k < 4; k++) __hip_atomic_store(&fixed[(long long)blockIdx.x * 4 + k], s[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __builtin_amdgcn_s_waitcnt(0);
+            last = __hip_atomic_fetch_add(out.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        }
+        __syncthreads();
+        if (!last) return;
+    }
+    double s[4] = {0, 0, 0, 0};
+    for (int i = threadIdx.x; i < nparts; i += 1024)
+        for (int k = 0; k < 4; k++) s[k] += out.partial[(long long)i * 4 + k];
+    if (out.near)
+        for (int i = threadIdx.x; i < (int)gridDim.x; i += 1024)
+            for (int k = 0; k < 4; k++) s[k] += __hip_atomic_load(&fixed[(long long)i * 4 + k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int o = 32; o > 0; o >>= 1)
+        for (int k = 0; k < 4; k++) s[k] += __shfl_xor(s[k], o);
+    if ((threadIdx.x & 63) == 0)
+        for (int k = 0; k < 4; k++) sh[threadIdx.x >> 6][k] = s[k];
+    __syncthreads();
+    if (threadIdx.x < 4) {
+        double v = 0.0;
+        for (int w = 0; w < 16; w++) v += sh[w][threadIdx.x];
+        sums[threadIdx.x] = (float)v;
     }
 }
 
@@ -514,8 +628,9 @@ int check_rows(const void *logits, int dtype, int64_t ldl, const int64_t *labels
     if (grad && overlap(logits, (size_t)M * ldl * dt_size(dtype), grad, (size_t)M * ldl * dt_size(grad_dtype))) return EMADAPT_ERR_INVALID;
     return EMADAPT_OK;
 }
-Rows rows_of(const void *logits, int64_t ldl, const int64_t *labels, int64_t M, int64_t C) {
-    return Rows{logits, reinterpret_cast<const long long *>(labels), (long long)ldl, (long long)M, (int)C};
+constexpr double kCache = 256e6;   // bytes of the last cache before the memory
+Rows rows_of(const void *logits, int64_t ldl, const int64_t *labels, int64_t M, int64_t C, size_t grad_size = 0) {
+    return Rows{logits, reinterpret_cast<const long long *>(labels), (long long)ldl, (long long)M, (int)C, (double)M * ldl * grad_size > kCache / 4};
 }
 
 // Rows of up to 64 vectors: as many lanes as vectors.  false: longer rows.
@@ -545,28 +660,36 @@ bool launch_block(const Rows &a, const Policy &p, const Outputs &out, int cap, i
     if (nvec > 16384) return false;
     *blocks = (int)grid_of(a.M, cap);
     const dim3 grid(*blocks);
-    if (nvec <= 128) hipLaunchKernelGGL((block_kernel<T, TD, 1, 2, MODE>), grid, dim3(64), 0, stream, a, p, out);
-    else if (nvec <= 256) hipLaunchKernelGGL((block_kernel<T, TD, 1, 4, MODE>), grid, dim3(64), 0, stream, a, p, out);
-    else if (nvec <= 1024) hipLaunchKernelGGL((block_kernel<T, TD, 4, 4, MODE>), grid, dim3(256), 0, stream, a, p, out);
-    else if (nvec <= 2048) hipLaunchKernelGGL((block_kernel<T, TD, 4, 8, MODE>), grid, dim3(256), 0, stream, a, p, out);
-    else if (nvec <= 4096) hipLaunchKernelGGL((block_kernel<T, TD, 8, 8, MODE>), grid, dim3(512), 0, stream, a, p, out);
-    else if (nvec <= 8192) hipLaunchKernelGGL((block_kernel<T, TD, 16, 8, MODE>), grid, dim3(1024), 0, stream, a, p, out);
-    else hipLaunchKernelGGL((block_kernel<T, TD, 16, 16, MODE>), grid, dim3(1024), 0, stream, a, p, out);
+#define EMADAPT_BLOCK(W, NV) hipLaunchKernelGGL((block_kernel<T, TD, W, NV, MODE>), grid, dim3(64 * W), 0, stream, a, p, out)
+    if (nvec <= 128) EMADAPT_BLOCK(1, 2);
+    else if (nvec <= 256) EMADAPT_BLOCK(1, 4);
+    else if (nvec <= 512) EMADAPT_BLOCK(1, 8);
+    else if (nvec <= 1024) EMADAPT_BLOCK(1, 16);
+    else if (nvec <= 2048) EMADAPT_BLOCK(2, 16);
+    else if (nvec <= 4096) EMADAPT_BLOCK(4, 16);
+    else if (nvec <= 8192) EMADAPT_BLOCK(8, 16);
+    else EMADAPT_BLOCK(16, 16);
+#undef EMADAPT_BLOCK
     return true;
 }
+inline int stats_width(int C) { return C <= 16384 ? 4 : 16; }   // waves to a row
+// again: the rows are read once more afterwards
 template <typename T>
-int launch_stats_t(const Rows &a, const Outputs &out, hipStream_t stream) {
+int launch_stats_t(const Rows &a, const Outputs &out, int splits, bool again, hipStream_t stream) {
     int blocks;
-    if (!launch_short<kLogp, T, T>(a, Policy(), out, 1 << 16, &blocks, stream)) {
-        // a workgroup wide enough to hold what a CU's share of the memory's rate needs in flight
-        const dim3 grid(grid_of(a.M, 1 << 16));
-        if (a.C <= 16384) hipLaunchKernelGGL((stream_stats_kernel<T, 4>), grid, dim3(256), 0, stream, a, out);
-        else hipLaunchKernelGGL((stream_stats_kernel<T, 16>), grid, dim3(1024), 0, stream, a, out);
+    if (splits > 1 || !launch_short<kLogp, T, T>(a, Policy(), out, 1 << 16, &blocks, stream)) {
+        // a workgroup wide enough to hold what a CU's share of the memory's rate needs in flight (rows of 32768 bf16: 95 us with 16 waves, 102 with 4)
+        const dim3 grid(grid_of(a.M, 1 << 16), splits);
+        const bool narrow = splits > 1 || stats_width(a.C) == 4;
+        if (narrow && again) hipLaunchKernelGGL((stream_stats_kernel<T, 4, false>), grid, dim3(256), 0, stream, a, out);
+        else if (narrow) hipLaunchKernelGGL((stream_stats_kernel<T, 4, true>), grid, dim3(256), 0, stream, a, out);
+        else if (again) hipLaunchKernelGGL((stream_stats_kernel<T, 16, false>), grid, dim3(1024), 0, stream, a, out);
+        else hipLaunchKernelGGL((stream_stats_kernel<T, 16, true>), grid, dim3(1024), 0, stream, a, out);
     }
     return launch_status();
 }
-int launch_stats(const Rows &a, int dtype, const Outputs &out, hipStream_t stream) {
-    return dtype == EMADAPT_DT_BF16 ? launch_stats_t<__bf16>(a, out, stream) : launch_stats_t<float>(a, out, stream);
+int launch_stats(const Rows &a, int dtype, const Outputs &out, bool again, hipStream_t stream) {
+    return dtype == EMADAPT_DT_BF16 ? launch_stats_t<__bf16>(a, out, 1, again, stream) : launch_stats_t<float>(a, out, 1, again, stream);
 }
 template <typename T>
 int launch_grad_t(const Rows &a, const float *base, const float *sum, const float *coef, void *d, int ddt, hipStream_t stream) {
@@ -582,31 +705,85 @@ int launch_grad(const Rows &a, int dtype, const float *base, const float *sum, c
 }
 constexpr int kPolicyBlocks = 2048;
 
-template <typename T>
-int policy_t(const Rows &a, const Policy &p, float *sums, float *logp, void *dlogits, int ddt, void *workspace, hipStream_t stream) {
-    float *base = static_cast<float *>(workspace), *sum = base + a.M, *coef = sum + a.M;
-    double *partial = reinterpret_cast<double *>(static_cast<char *>(workspace) + align_up((size_t)a.M * 12, 256));
-    const Outputs out = {logp, nullptr, nullptr, nullptr, nullptr, dlogits, partial};
+#ifndef FEWROWS
+#define FEWROWS kFewRows
+#endif
+#ifndef FEWVEC
+#define FEWVEC 4096
+#endif
+constexpr int kSplits = 32;
+// Where the policy loss keeps what its launches hand on.
+struct PolicySpace {
+    float *base, *sum, *coef;   // [M] each
+    MaxSum *parts;              // [kFewRows][kSplits]
+    double *partial, *fixed;    // [kPolicyBlocks][4], [ceil(M / 1024)][4]
+    unsigned *ticket;
+    unsigned char *near;        // [M]
+    size_t bytes;
+};
+constexpr int64_t kFewRows = 128;
+PolicySpace policy_space(void *workspace, int64_t M) {
+    PolicySpace s;
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        char *p = static_cast<char *>(workspace) + at;
+        at += align_up(n, 256);
+        return p;
+    };
+    s.base = reinterpret_cast<float *>(take((size_t)M * 12));
+    s.sum = s.base + M;
+    s.coef = s.sum + M;
+    s.parts = reinterpret_cast<MaxSum *>(take(kFewRows * kSplits * sizeof(MaxSum)));
+    s.partial = reinterpret_cast<double *>(take((size_t)kPolicyBlocks * 32));
+    s.fixed = reinterpret_cast<double *>(take((size_t)ceil_div(M, 1024) * 32));
+    s.ticket = reinterpret_cast<unsigned *>(take(4));
+    s.near = reinterpret_cast<unsigned char *>(take((size_t)M));
+    s.bytes = at;
+    return s;
+}
+
+template <typename T, typename TD>
+int policy_t(const Rows &a, Policy p, float *sums, float *logp, void *dlogits, int ddt, void *workspace, hipStream_t stream) {
+    const PolicySpace w = policy_space(workspace, a.M);
+    Outputs out = {logp, nullptr, nullptr, nullptr, nullptr, dlogits, w.partial, nullptr, w.ticket, nullptr};
     int blocks = 0;
+    unsigned finish = 1;
     if (a.M) {
+        const int64_t nvec = a.C / Vec<T>::N;
+        const bool few = a.M <= FEWROWS && nvec > FEWVEC;   // (a CU to a row leaves the others idle)
         bool done;
+        p.tol = border_tol(16, (int)a.C);   // (short rows: none; a row in registers: 16 vectors to a thread)
         if (!dlogits) done = launch_short<kPolicy, T, T>(a, p, out, kPolicyBlocks, &blocks, stream);
-        else if (ddt == EMADAPT_DT_BF16)
-            done = launch_short<kPolicyGrad, T, __bf16>(a, p, out, kPolicyBlocks, &blocks, stream) || launch_block<kPolicyGrad, T, __bf16>(a, p, out, kPolicyBlocks, &blocks, stream);
-        else
-            done = launch_short<kPolicyGrad, T, float>(a, p, out, kPolicyBlocks, &blocks, stream) || launch_block<kPolicyGrad, T, float>(a, p, out, kPolicyBlocks, &blocks, stream);
+        else {
+            done = launch_short<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
+            if (!done && !few) {
+                out.near = w.near;
+                done = launch_block<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
+                if (done) finish = (unsigned)ceil_div(a.M, 1024);
+                else out.near = nullptr;
+            }
+        }
         if (int rc = launch_status()) return rc;
-        if (!done) {   // rows that no workgroup's registers hold, or that are only read: log-sum-exp, the rows' terms, the gradient
-            if (int rc = launch_stats_t<T>(a, Outputs{nullptr, nullptr, base, sum, nullptr, nullptr, nullptr}, stream)) return rc;
+        if (!done) {   // rows that no workgroup's registers hold, that are only read, or too few: log-sum-exp, the rows' terms, the gradient
+            Outputs st = {};
+            p.tol = border_tol((int)ceil_div(a.C, few ? kSplits * 256 * Vec<T>::N : stats_width(a.C) * 64 * Vec<T>::N) + (few ? kSplits : 0), (int)a.C);
+            if (few) st.parts = w.parts;
+            else { st.base = w.base; st.sum = w.sum; }
+            if (int rc = launch_stats_t<T>(a, st, few ? kSplits : 1, dlogits != nullptr, stream)) return rc;
             blocks = (int)grid_of(ceil_div(a.M, 256), kPolicyBlocks);
-            hipLaunchKernelGGL(policy_row_kernel<T>, dim3(blocks), dim3(256), 0, stream, a, p, base, sum, logp, coef, partial);
+            hipLaunchKernelGGL(policy_row_kernel<T>, dim3(blocks), dim3(256), 0, stream, a, p, st.parts, kSplits, w.base, w.sum, logp, w.coef, w.partial, sums);
             if (int rc = launch_status()) return rc;
             if (dlogits)
-                if (int rc = launch_grad_t<T>(a, base, sum, coef, dlogits, ddt, stream)) return rc;
+                if (int rc = launch_grad_t<T>(a, w.base, w.sum, w.coef, dlogits, ddt, stream)) return rc;
+            if (blocks == 1) return EMADAPT_OK;
         }
     }
-    hipLaunchKernelGGL(policy_sums_kernel, dim3(1), dim3(256), 0, stream, partial, blocks, sums);
+    hipLaunchKernelGGL((policy_finish_kernel<T, TD>), dim3(finish), dim3(1024), 0, stream, a, p, out, blocks, w.fixed, sums);
     return launch_status();
+}
+template <typename T>
+int policy_any(const Rows &a, const Policy &p, float *sums, float *logp, void *dlogits, int ddt, void *workspace, hipStream_t stream) {
+    return ddt == EMADAPT_DT_BF16 ? policy_t<T, __bf16>(a, p, sums, logp, dlogits, ddt, workspace, stream) : policy_t<T, float>(a, p, sums, logp, dlogits, ddt, workspace, stream);
 }
 
 }  // namespace
@@ -626,7 +803,10 @@ int emadapt_label_logp(const void *logits, int dtype, int64_t ldl, const int64_t
     if (!logp && !lse) return EMADAPT_ERR_INVALID;
     hipStream_t stream = as_stream(stream_);
     ProfScope prof(EMADAPT_K_OTHER, 0.0, (double)M * ((double)C * dt_size(dtype) + 16.0), stream);
-    return launch_stats(rows_of(logits, ldl, labels, M, C), dtype, Outputs{logp, lse, nullptr, nullptr, nullptr, nullptr, nullptr}, stream);
+    // (whether a gradient follows is not known here: of up to twice the cache a second reader still finds a good part -- 4001 x 32768 bf16 with
+    // the gradient 127 us, 138 where the first reader leaves nothing; 1500 x 100003 f32 alone 98 and 92)
+    const bool again = (double)M * C * dt_size(dtype) < 2 * kCache;
+    return launch_stats(rows_of(logits, ldl, labels, M, C), dtype, Outputs{logp, lse}, again, stream);
 }
 
 int emadapt_label_logp_bwd(const void *logits, int dtype, int64_t ldl, const int64_t *labels, const float *lse, const float *dlogp, int64_t M, int64_t C,
@@ -636,12 +816,12 @@ int emadapt_label_logp_bwd(const void *logits, int dtype, int64_t ldl, const int
     if (!lse || !dlogp || !dlogits) return EMADAPT_ERR_INVALID;
     hipStream_t stream = as_stream(stream_);
     ProfScope prof(EMADAPT_K_OTHER, 0.0, (double)M * ((double)C * dt_size(dtype) + (double)ldl * dt_size(dlogits_dtype) + 16.0), stream);
-    return launch_grad(rows_of(logits, ldl, labels, M, C), dtype, lse, nullptr, dlogp, dlogits, dlogits_dtype, stream);
+    return launch_grad(rows_of(logits, ldl, labels, M, C, dt_size(dlogits_dtype)), dtype, lse, nullptr, dlogp, dlogits, dlogits_dtype, stream);
 }
 
 size_t emadapt_policy_loss_workspace_bytes(int64_t M, int64_t C) {
     (void)C;
-    return align_up((size_t)(M > 0 ? M : 0) * 12, 256) + (size_t)kPolicyBlocks * 4 * sizeof(double);
+    return policy_space(nullptr, M > 0 ? M : 0).bytes;
 }
 
 int emadapt_policy_loss(const void *logits, int dtype, int64_t ldl, const int64_t *actions, const float *old_logp, const float *ref_logp, const float *advantages,
@@ -653,10 +833,10 @@ int emadapt_policy_loss(const void *logits, int dtype, int64_t ldl, const int64_
     if (!workspace || !aligned(workspace, 8) || workspace_bytes < emadapt_policy_loss_workspace_bytes(M, C)) return EMADAPT_ERR_WORKSPACE;
     hipStream_t stream = as_stream(stream_);
     ProfScope prof(EMADAPT_K_OTHER, 0.0, (double)M * ((double)C * dt_size(dtype) + (dlogits ? (double)ldl * dt_size(dlogits_dtype) : 0.0) + 28.0), stream);
-    const Rows a = rows_of(logits, ldl, actions, M, C);
-    const Policy p = {old_logp, ref_logp, advantages, weights, 1.0 - clip_low, 1.0 + clip_high, log1p(-clip_low), log1p(clip_high), kl_coef, grad_scale};
-    return dtype == EMADAPT_DT_BF16 ? policy_t<__bf16>(a, p, sums, logp, dlogits, dlogits_dtype, workspace, stream)
-                                    : policy_t<float>(a, p, sums, logp, dlogits, dlogits_dtype, workspace, stream);
+    const Rows a = rows_of(logits, ldl, actions, M, C, dt_size(dlogits_dtype));
+    const Policy p = {old_logp, ref_logp, advantages, weights, 1.0 - clip_low, 1.0 + clip_high, log1p(-clip_low), log1p(clip_high), kl_coef, grad_scale, 0.f};
+    return dtype == EMADAPT_DT_BF16 ? policy_any<__bf16>(a, p, sums, logp, dlogits, dlogits_dtype, workspace, stream)
+                                    : policy_any<float>(a, p, sums, logp, dlogits, dlogits_dtype, workspace, stream);
 }
 
 size_t emadapt_preference_loss_workspace_bytes(int64_t M, int64_t C) {
@@ -675,9 +855,9 @@ int emadapt_preference_loss(const void *logits, int dtype, int64_t ldl, const in
     hipStream_t stream = as_stream(stream_);
     ProfScope prof(EMADAPT_K_OTHER, 0.0, (double)M * (2.0 * C * dt_size(dtype) + (dlogits ? (double)ldl * dt_size(dlogits_dtype) : 0.0) + 24.0), stream);
     float *logp = static_cast<float *>(workspace), *base = logp + M, *sum = base + M, *coef = sum + M;
-    const Rows a = rows_of(logits, ldl, labels, M, C);
+    const Rows a = rows_of(logits, ldl, labels, M, C, dt_size(dlogits_dtype));
     if (M)   // (rows of no sequence have no gradient: their coefficient starts at 0)
-        if (int rc = launch_stats(a, dtype, Outputs{logp, nullptr, dlogits ? base : nullptr, sum, dlogits ? coef : nullptr, nullptr, nullptr}, stream)) return rc;
+        if (int rc = launch_stats(a, dtype, Outputs{logp, nullptr, dlogits ? base : nullptr, sum, dlogits ? coef : nullptr}, dlogits != nullptr, stream)) return rc;
     if (pairs) {
         hipLaunchKernelGGL(preference_pair_kernel, dim3((unsigned)pairs), dim3(1024), 0, stream, logp, reinterpret_cast<const long long *>(seq_start), ref_logp, (long long)M,
                            beta, label_smoothing, grad_scale, loss, seq_logp, dlogits ? coef : nullptr);
