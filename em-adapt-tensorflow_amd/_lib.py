@@ -156,8 +156,7 @@ PROTOTYPES = {
     "emadapt_sgd_accumulate_pack": (c_int, [_vp, _vp, c_int64, c_int64, c_float, c_float, _vp, c_int, _vp]),
     "emadapt_grad_pack": (c_int, [_vp, c_int64, _vp, c_int, c_int64, _vp]),
     "emadapt_grad_owner_sum": (c_int, [_vp, c_int, c_int, c_int64, _vp, _vp]),
-    "emadapt_label_logp_workspace_bytes": (c_size_t, [c_int64, c_int64]),
-    "emadapt_label_logp": (c_int, [_vp, c_int, c_int64, _vp, c_int64, c_int64, _vp, _vp, _vp, c_size_t, _vp]),
+    "emadapt_label_logp": (c_int, [_vp, c_int, c_int64, _vp, c_int64, c_int64, _vp, _vp, _vp]),
     "emadapt_label_logp_bwd": (c_int, [_vp, c_int, c_int64, _vp, _vp, _vp, c_int64, c_int64, _vp, c_int, _vp]),
     "emadapt_policy_loss_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "emadapt_policy_loss": (c_int, [_vp, c_int, c_int64, _vp, _vp, _vp, _vp, _vp, c_int64, c_int64, c_double, c_double, c_float, c_float, _vp,

@@ -119,15 +119,12 @@ struct Rows {
     long long ldl, M;
     int C;
     bool once;   // the gradient is too large to stay in the cache: it is not left there
+    bool last;   // nor are the logits, which are read for the last time
 };
 
-// dz = [c = label] coef - exp(z - base) coef / sum (base, sum: the row's maximum and sum; without sum the log-sum-exp): every thread its vectors of the flattened [M][vectors per row], kUnroll of them in flight.  A
+// dz = [c = label] coef - exp(z - base) coef / sum (base, sum: the row's maximum and sum; without sum the log-sum-exp): every thread kUnroll vectors of the flattened [M][vectors per row], all in flight.  A
 // workgroup's vectors lie behind one another; their rows come from one 64-bit division for the workgroup and a 32-bit one for each vector.
-#ifndef GONCE
-#define GONCE true
-#endif
-constexpr int kUnroll = 4;
-template <typename T, typename TD>
+template <typename T, typename TD, int kUnroll>
 __global__ void __launch_bounds__(256) row_grad_kernel(Rows a, const float *__restrict__ base, const float *__restrict__ sum, const float *__restrict__ coef, TD *__restrict__ dlogits,
                                                       unsigned nvec, long long total) {
     constexpr int N = Vec<T>::N;
@@ -144,7 +141,7 @@ __global__ void __launch_bounds__(256) row_grad_kernel(Rows a, const float *__re
         row[q] = b + q * 256 + threadIdx.x < total ? r0 + dr : -1;
         if (row[q] < 0) continue;
         at[q] = (int)(o - dr * nvec) * N;
-        raw[q] = load_row<GONCE>(static_cast<const T *>(a.logits) + row[q] * a.ldl, at[q], a.C, (int)a.ldl);
+        raw[q] = load_row<false>(static_cast<const T *>(a.logits) + row[q] * a.ldl, at[q], a.C, (int)a.ldl);
         const long long lab = a.labels[row[q]];
         const bool used = lab >= 0 && lab < a.C;
         hit[q] = used ? (int)lab : -(1 << 30);
@@ -227,6 +224,7 @@ __device__ double exact_part(const T *z, int C, long long lab, int first, int st
 // rows that stay in registers: one pass over the logits
 // ------------------------------------------------------------------------------------------
 enum { kLogp = 0, kPolicy = 1, kPolicyGrad = 2 };
+constexpr int kSplits = 32;   // parts of a row where rows are few
 struct Outputs {
     float *logp, *lse;          // kLogp: any of these may be null
     float *base, *sum, *zero;   // kLogp: the rows' maximum and sum of exponentials; a value per row set to 0
@@ -257,8 +255,9 @@ __device__ __forceinline__ float policy_of_exact(const Policy &p, const PolicyIn
     return policy_row((float)lr, (float)((double)x.refp - lp64), x.has_ref, x.adv, x.w, p, past_border(lr, x.adv, p), count, t);
 }
 
-// L lanes to a row, a vector of the padded row to a lane.
-template <typename T, typename TD, int L, int MODE>
+// L lanes to a row, NV vectors of the padded row to a lane: few lanes, so that what is done once a row (logarithm, loss) is done for many rows by
+// a wave's instruction (1.6 M rows of 24 f32: 54 us with a vector to a lane, 39 with three).
+template <typename T, typename TD, int L, int NV, int MODE>
 __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs out) {
     constexpr int N = Vec<T>::N;
     __shared__ double sh[4];
@@ -268,25 +267,47 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
     for (long long r = (long long)blockIdx.x * (256 / L) + threadIdx.x / L; r < a.M; r += per_grid) {
         const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
         const long long lab = a.labels[r];
-        bool used = lab >= 0 && lab < a.C;
-        if (MODE != kLogp && p.weight) used = used && p.weight[r] != 0.f;
-        const int i = lane * N;
-        const Raw raw = load_row<MODE != kLogp>(z, i, a.C, (int)a.ldl);
-        float v[N], m = -INFINITY, s = 0.f;
-        unpack<T>(raw, v);
+        PolicyInputs x = {0.f, 0.f, 1.f, 0.f, false};
+        if (MODE != kLogp) x = policy_inputs(p, r);   // (in front of the row: their way to memory is the row's)
+        const bool used = lab >= 0 && lab < a.C && x.w != 0.f;
+        const float zl = (float)z[used ? lab : 0];
+        Raw raw[NV];
+        if (a.last) {
+            asm volatile("");
 #pragma unroll
-        for (int e = 0; e < N; e++) m = fmaxf(m, v[e]);
+            for (int k = 0; k < NV; k++) raw[k] = load_row<true>(z, (lane + k * L) * N, a.C, (int)a.ldl);
+            asm volatile("");
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV; k++) raw[k] = load_row<false>(z, (lane + k * L) * N, a.C, (int)a.ldl);
+        }
+        float m = -INFINITY, s = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            float v[N];
+            unpack<T>(raw[k], v);
+#pragma unroll
+            for (int e = 0; e < N; e++) m = fmaxf(m, v[e]);
+        }
         m = group_max<L>(m);
         const float m0 = finite_or_0(m);
 #pragma unroll
-        for (int e = 0; e < N; e++) s += __expf(v[e] - m0);
+        for (int k = 0; k < NV; k++) {
+            float v[N];
+            unpack<T>(raw[k], v);
+#pragma unroll
+            for (int e = 0; e < N; e++) v[e] = __expf(v[e] - m0);
+#pragma unroll
+            for (int w = N / 2; w > 0; w /= 2)
+#pragma unroll
+                for (int e = 0; e < w; e++) v[e] += v[e + w];
+            s += v[0];
+        }
         s = group_sum<L>(s);
         float lp = 0.f, f = 0.f;
         if (used) {
-            const float zl = (float)z[lab];
             if (MODE == kLogp) lp = (float)logp_of(zl, MaxSum{m, s});
             else {
-                const PolicyInputs x = policy_inputs(p, r);
                 bool near;
                 f = policy_of_row(p, x, zl, MaxSum{m, s}, lane == 0, lp, near, t);
                 if (near) {
@@ -304,13 +325,20 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
                 if (out.zero) out.zero[r] = 0.f;
             }
         }
-        if (MODE == kPolicyGrad && i < a.ldl) {
-            grad_vec<T>(raw, m, f * __builtin_amdgcn_rcpf(s), f, used ? (int)lab - i : -1, v);
-            if (f == 0.f) {
+        if (MODE == kPolicyGrad) {
+            const float fs = f * __builtin_amdgcn_rcpf(s);
 #pragma unroll
-                for (int e = 0; e < N; e++) v[e] = 0.f;
+            for (int k = 0; k < NV; k++) {
+                const int i = (lane + k * L) * N;
+                if (i >= a.ldl) continue;
+                float v[N];
+                grad_vec<T>(raw[k], m, fs, f, used ? (int)lab - i : -1, v);
+                if (f == 0.f) {
+#pragma unroll
+                    for (int e = 0; e < N; e++) v[e] = 0.f;
+                }
+                store_row<TD>(static_cast<TD *>(out.dlogits) + r * a.ldl, i, (int)a.ldl, v, a.once);
             }
-            store_row<TD>(static_cast<TD *>(out.dlogits) + r * a.ldl, i, (int)a.ldl, v, a.once);
         }
     }
     if (MODE != kLogp) {
@@ -465,31 +493,35 @@ __global__ void __launch_bounds__(64 * W) stream_stats_kernel(Rows a, Outputs ou
     }
 }
 
-// The rows' terms where the log-sum-exp comes from a launch of its own, as the rows' maximum and sum or in `splits` parts of each row.  One
+// The rows' terms where the log-sum-exp comes from a launch of its own, as the rows' maximum and sum or in kSplits parts of each row.  One
 // workgroup also writes the sums.
 template <typename T>
-__global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const MaxSum *__restrict__ parts, int splits, float *__restrict__ base,
+__global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const MaxSum *__restrict__ parts, float *__restrict__ base,
                                                         float *__restrict__ sum, float *__restrict__ logp, float *__restrict__ coef,
                                                         double *__restrict__ partial, float *__restrict__ sums) {
     __shared__ double sh[4];
     __shared__ unsigned long long mask[4];
+    __shared__ MaxSum whole[256];
     PolicyTerms t = {0, 0, 0, 0};
     for (long long r0 = (long long)blockIdx.x * 256; r0 < a.M; r0 += (long long)gridDim.x * 256) {
         const long long r = r0 + threadIdx.x;
         bool again = false;
+        if (parts) {   // a lane to a part, kSplits of them to a row
+            for (int q = threadIdx.x / kSplits; q < 256 && r0 + q < a.M; q += 256 / kSplits) {
+                const MaxSum part = parts[(r0 + q) * kSplits + threadIdx.x % kSplits];
+                const float m = group_max<kSplits>(part.m), s = group_sum<kSplits>(part.s * __expf(part.m - finite_or_0(m)));
+                if (threadIdx.x % kSplits == 0) {
+                    whole[q] = {m, s};
+                    base[r0 + q] = m;
+                    sum[r0 + q] = s;
+                }
+            }
+            __syncthreads();
+        }
         if (r < a.M) {
             const long long lab = a.labels[r];
             const float w = p.weight ? p.weight[r] : 1.f;
-            MaxSum row;
-            if (parts) {
-                row = parts[r * splits];
-                for (int k = 1; k < splits; k++) row.m = fmaxf(row.m, parts[r * splits + k].m);
-                row.s = 0.f;
-                for (int k = 0; k < splits; k++) row.s += parts[r * splits + k].s * __expf(parts[r * splits + k].m - finite_or_0(row.m));
-                base[r] = row.m;
-                sum[r] = row.s;
-            } else
-                row = {base[r], sum[r]};
+            const MaxSum row = parts ? whole[threadIdx.x] : MaxSum{base[r], sum[r]};
             float lp = 0.f, f = 0.f;
             if (lab >= 0 && lab < a.C && w != 0.f)
                 f = policy_of_row(p, policy_inputs(p, r), (float)(static_cast<const T *>(a.logits) + r * a.ldl)[lab], row, true, lp, again, t);
@@ -630,27 +662,27 @@ int check_rows(const void *logits, int dtype, int64_t ldl, const int64_t *labels
 }
 constexpr double kCache = 256e6;   // bytes of the last cache before the memory
 Rows rows_of(const void *logits, int64_t ldl, const int64_t *labels, int64_t M, int64_t C, size_t grad_size = 0) {
-    return Rows{logits, reinterpret_cast<const long long *>(labels), (long long)ldl, (long long)M, (int)C, (double)M * ldl * grad_size > kCache / 4};
+    return Rows{logits, reinterpret_cast<const long long *>(labels), (long long)ldl, (long long)M, (int)C, (double)M * ldl * grad_size > kCache / 4, false};
 }
 
-// Rows of up to 64 vectors: as many lanes as vectors.  false: longer rows.
+// Rows of up to 64 vectors, three or four of them to a lane.  false: longer rows.
 template <int MODE, typename T, typename TD>
 bool launch_short(const Rows &a, const Policy &p, const Outputs &out, int cap, int *blocks, hipStream_t stream) {
     const int64_t nvec = ceil_div(a.ldl, Vec<T>::N);
     if (nvec > 64) return false;
     int L = 1;
-    while (L < nvec) L *= 2;
+    while (L * 4 < nvec) L *= 2;
+    const bool three = nvec <= 3 * L;
     *blocks = (int)grid_of(ceil_div(a.M, 256 / L), cap);
-    const dim3 grid(*blocks), block(256);
+#define EMADAPT_GROUP(L, NV) hipLaunchKernelGGL((group_kernel<T, TD, L, NV, MODE>), dim3(*blocks), dim3(256), 0, stream, a, p, out)
     switch (L) {
-        case 1: hipLaunchKernelGGL((group_kernel<T, TD, 1, MODE>), grid, block, 0, stream, a, p, out); break;
-        case 2: hipLaunchKernelGGL((group_kernel<T, TD, 2, MODE>), grid, block, 0, stream, a, p, out); break;
-        case 4: hipLaunchKernelGGL((group_kernel<T, TD, 4, MODE>), grid, block, 0, stream, a, p, out); break;
-        case 8: hipLaunchKernelGGL((group_kernel<T, TD, 8, MODE>), grid, block, 0, stream, a, p, out); break;
-        case 16: hipLaunchKernelGGL((group_kernel<T, TD, 16, MODE>), grid, block, 0, stream, a, p, out); break;
-        case 32: hipLaunchKernelGGL((group_kernel<T, TD, 32, MODE>), grid, block, 0, stream, a, p, out); break;
-        default: hipLaunchKernelGGL((group_kernel<T, TD, 64, MODE>), grid, block, 0, stream, a, p, out);
+        case 1: if (three) EMADAPT_GROUP(1, 3); else EMADAPT_GROUP(1, 4); break;
+        case 2: if (three) EMADAPT_GROUP(2, 3); else EMADAPT_GROUP(2, 4); break;
+        case 4: if (three) EMADAPT_GROUP(4, 3); else EMADAPT_GROUP(4, 4); break;
+        case 8: if (three) EMADAPT_GROUP(8, 3); else EMADAPT_GROUP(8, 4); break;
+        default: if (three) EMADAPT_GROUP(16, 3); else EMADAPT_GROUP(16, 4);
     }
+#undef EMADAPT_GROUP
     return true;
 }
 // Rows of up to 16384 vectors in the registers of a workgroup.
@@ -675,8 +707,9 @@ bool launch_block(const Rows &a, const Policy &p, const Outputs &out, int cap, i
 inline int stats_width(int C) { return C <= 16384 ? 4 : 16; }   // waves to a row
 // again: the rows are read once more afterwards
 template <typename T>
-int launch_stats_t(const Rows &a, const Outputs &out, int splits, bool again, hipStream_t stream) {
+int launch_stats_t(Rows a, const Outputs &out, int splits, bool again, hipStream_t stream) {
     int blocks;
+    a.last = !again;
     if (splits > 1 || !launch_short<kLogp, T, T>(a, Policy(), out, 1 << 16, &blocks, stream)) {
         // a workgroup wide enough to hold what a CU's share of the memory's rate needs in flight (rows of 32768 bf16: 95 us with 16 waves, 102 with 4)
         const dim3 grid(grid_of(a.M, 1 << 16), splits);
@@ -693,11 +726,19 @@ int launch_stats(const Rows &a, int dtype, const Outputs &out, bool again, hipSt
 }
 template <typename T>
 int launch_grad_t(const Rows &a, const float *base, const float *sum, const float *coef, void *d, int ddt, hipStream_t stream) {
-    const int64_t nvec = ceil_div(a.ldl, Vec<T>::N), total = nvec * a.M, blocks = ceil_div(total, 256 * kUnroll);
+    const int64_t nvec = ceil_div(a.ldl, Vec<T>::N), total = nvec * a.M;
+    // four vectors to a thread, or one where that leaves CUs without a workgroup (40344 rows of 24 f32: 7.7 us and 4.1)
+    const bool four = total >= 4 * 256 * 1024;
+    const int64_t blocks = ceil_div(total, four ? 1024 : 256);
     if (blocks > 0x7FFFFFFF) return EMADAPT_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)blocks);
-    if (ddt == EMADAPT_DT_BF16) hipLaunchKernelGGL((row_grad_kernel<T, __bf16>), grid, dim3(256), 0, stream, a, base, sum, coef, static_cast<__bf16 *>(d), (unsigned)nvec, (long long)total);
-    else hipLaunchKernelGGL((row_grad_kernel<T, float>), grid, dim3(256), 0, stream, a, base, sum, coef, static_cast<float *>(d), (unsigned)nvec, (long long)total);
+#define EMADAPT_GRAD(TD, U) \
+    hipLaunchKernelGGL((row_grad_kernel<T, TD, U>), dim3((unsigned)blocks), dim3(256), 0, stream, a, base, sum, coef, static_cast<TD *>(d), (unsigned)nvec, (long long)total)
+    if (ddt == EMADAPT_DT_BF16) {
+        if (four) EMADAPT_GRAD(__bf16, 4); else EMADAPT_GRAD(__bf16, 1);
+    } else {
+        if (four) EMADAPT_GRAD(float, 4); else EMADAPT_GRAD(float, 1);
+    }
+#undef EMADAPT_GRAD
     return launch_status();
 }
 int launch_grad(const Rows &a, int dtype, const float *base, const float *sum, const float *coef, void *d, int ddt, hipStream_t stream) {
@@ -705,13 +746,6 @@ int launch_grad(const Rows &a, int dtype, const float *base, const float *sum, c
 }
 constexpr int kPolicyBlocks = 2048;
 
-#ifndef FEWROWS
-#define FEWROWS kFewRows
-#endif
-#ifndef FEWVEC
-#define FEWVEC 4096
-#endif
-constexpr int kSplits = 32;
 // Where the policy loss keeps what its launches hand on.
 struct PolicySpace {
     float *base, *sum, *coef;   // [M] each
@@ -743,15 +777,16 @@ PolicySpace policy_space(void *workspace, int64_t M) {
 }
 
 template <typename T, typename TD>
-int policy_t(const Rows &a, Policy p, float *sums, float *logp, void *dlogits, int ddt, void *workspace, hipStream_t stream) {
+int policy_t(Rows a, Policy p, float *sums, float *logp, void *dlogits, int ddt, void *workspace, hipStream_t stream) {
     const PolicySpace w = policy_space(workspace, a.M);
     Outputs out = {logp, nullptr, nullptr, nullptr, nullptr, dlogits, w.partial, nullptr, w.ticket, nullptr};
     int blocks = 0;
     unsigned finish = 1;
     if (a.M) {
         const int64_t nvec = a.C / Vec<T>::N;
-        const bool few = a.M <= FEWROWS && nvec > FEWVEC;   // (a CU to a row leaves the others idle)
+        const bool few = a.M <= kFewRows && nvec > 4096;   // (a CU to a row leaves the others idle)
         bool done;
+        a.last = a.once;
         p.tol = border_tol(16, (int)a.C);   // (short rows: none; a row in registers: 16 vectors to a thread)
         if (!dlogits) done = launch_short<kPolicy, T, T>(a, p, out, kPolicyBlocks, &blocks, stream);
         else {
@@ -771,7 +806,7 @@ int policy_t(const Rows &a, Policy p, float *sums, float *logp, void *dlogits, i
             else { st.base = w.base; st.sum = w.sum; }
             if (int rc = launch_stats_t<T>(a, st, few ? kSplits : 1, dlogits != nullptr, stream)) return rc;
             blocks = (int)grid_of(ceil_div(a.M, 256), kPolicyBlocks);
-            hipLaunchKernelGGL(policy_row_kernel<T>, dim3(blocks), dim3(256), 0, stream, a, p, st.parts, kSplits, w.base, w.sum, logp, w.coef, w.partial, sums);
+            hipLaunchKernelGGL(policy_row_kernel<T>, dim3(blocks), dim3(256), 0, stream, a, p, st.parts, w.base, w.sum, logp, w.coef, w.partial, sums);
             if (int rc = launch_status()) return rc;
             if (dlogits)
                 if (int rc = launch_grad_t<T>(a, w.base, w.sum, w.coef, dlogits, ddt, stream)) return rc;
@@ -790,14 +825,7 @@ int policy_any(const Rows &a, const Policy &p, float *sums, float *logp, void *d
 
 extern "C" {
 
-size_t emadapt_label_logp_workspace_bytes(int64_t M, int64_t C) {
-    (void)M; (void)C;
-    return 0;
-}
-
-int emadapt_label_logp(const void *logits, int dtype, int64_t ldl, const int64_t *labels, int64_t M, int64_t C, float *logp, float *lse, void *workspace,
-                       size_t workspace_bytes, void *stream_) {
-    (void)workspace; (void)workspace_bytes;
+int emadapt_label_logp(const void *logits, int dtype, int64_t ldl, const int64_t *labels, int64_t M, int64_t C, float *logp, float *lse, void *stream_) {
     if (int rc = check_rows(logits, dtype, ldl, labels, M, C, nullptr, 0)) return rc;
     if (M == 0) return EMADAPT_OK;
     if (!logp && !lse) return EMADAPT_ERR_INVALID;

@@ -4,7 +4,6 @@ torch provides device memory and the current HIP stream; every computation happe
 libemadapt_hip.so.  All tensors are fp32, NHWC, contiguous; filters are HWIO like the reference's
 ``tf.get_variable`` shapes (deeplab.py:131-149).
 """
-import contextlib
 import ctypes
 
 import torch
@@ -830,27 +829,14 @@ def grad_owner_sum(recv, world, out):
 
 
 # ---- losses over the log-probability of given labels (include/emadapt.h, "Losses over the log-probability ...")
-def _rows(logits, labels, num_classes, name="labels"):
-    """Checks logits [..., ldl] f32 / bf16 with labels int64 [...]; returns (dtype code, ldl, rows)."""
-    dt = _float_dt(logits, "logits")
-    _check(labels, torch.int64, name)
-    if logits.dim() < 1:
-        raise ValueError("logits must be [..., classes]")
-    ldl = logits.shape[-1]
-    if not 0 < int(num_classes) <= ldl:
-        raise ValueError("num_classes %d does not fit logits of %d columns" % (num_classes, ldl))
-    M = labels.numel()
-    if tuple(labels.shape) != tuple(logits.shape[:-1]):
-        raise ValueError("%s has shape %s, the logits' rows %s" % (name, tuple(labels.shape), tuple(logits.shape[:-1])))
-    _same_device(logits, labels, name)
-    return dt, ldl, M
+_DT_OF = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
 
 
 def _float_dt(t, name):
     """EMADAPT_DT_* of a contiguous f32 / bf16 GPU tensor of any shape."""
     if not t.is_cuda:
         raise ValueError("%s must live on the GPU (there is no CPU path)" % name)
-    dt = DT_F32 if t.dtype == torch.float32 else DT_BF16 if t.dtype == torch.bfloat16 else None
+    dt = _DT_OF.get(t.dtype)
     if dt is None:
         raise TypeError("%s must be float32 or bfloat16, got %s" % (name, t.dtype))
     if not t.is_contiguous():
@@ -859,22 +845,40 @@ def _float_dt(t, name):
 
 
 def _same_device(a, b, name):
-    if b.device != a.device:
+    if b.get_device() != a.get_device():
         raise ValueError("%s lives on %s, the logits on %s" % (name, b.device, a.device))
 
 
+def _rows(logits, labels, num_classes, name="labels"):
+    """Checks logits [..., ldl] f32 / bf16 with labels int64 [...]; returns (dtype code, ldl, rows, classes)."""
+    dt = _float_dt(logits, "logits")
+    _check(labels, torch.int64, name)
+    shape = logits.shape
+    if not shape:
+        raise ValueError("logits must be [..., classes]")
+    if labels.shape != shape[:-1]:
+        raise ValueError("%s has shape %s, the logits' rows %s" % (name, tuple(labels.shape), tuple(shape[:-1])))
+    C = int(num_classes)
+    if not 0 < C <= shape[-1]:
+        raise ValueError("num_classes %d does not fit logits of %d columns" % (C, shape[-1]))
+    _same_device(logits, labels, name)
+    return dt, shape[-1], labels.numel(), C
+
+
 def _row_vector(t, logits, M, name):
-    """An f32 value per row (or None)."""
-    if t is not None:
-        _check(t, name=name)
-        if t.numel() != M:
-            raise ValueError("%s holds %d values, the logits %d rows" % (name, t.numel(), M))
-        _same_device(logits, t, name)
+    """Address of an f32 value per row (or None)."""
+    if t is None:
+        return None
+    _check(t, name=name)
+    if t.numel() != M:
+        raise ValueError("%s holds %d values, the logits %d rows" % (name, t.numel(), M))
+    _same_device(logits, t, name)
+    return t.data_ptr()
 
 
-def _dlogits(logits, dlogits):
+def _dlogits(logits, dt, dlogits):
     if dlogits is None:
-        return torch.empty_like(logits), _float_dt(logits, "dlogits")
+        return torch.empty_like(logits), dt
     ddt = _float_dt(dlogits, "dlogits")
     if dlogits.shape != logits.shape:
         raise ValueError("dlogits must have the logits' shape")
@@ -882,38 +886,44 @@ def _dlogits(logits, dlogits):
     return dlogits, ddt
 
 
-def _scratch(nbytes, t):
+def _f32(shape, like):
+    return torch.empty(shape, dtype=torch.float32, device=like.device)
+
+
+def _scratch(nbytes, like):
     """Workspace of one call, from torch's allocator (not the shared one): calls on several streams and captured graphs never share it."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
 
 
-def _on(t):
-    """The launches go to the tensors' device, whichever is current."""
-    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+def _launch(t, name, *args):
+    """Call an entry on the current stream of the tensor's device, whichever device is current; the stream goes last."""
+    index = t.get_device()
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _launch(t, name, *args)
+    rc = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        raise _lib.EmadaptError(rc, name)
 
 
 def label_logp(logits, labels, num_classes):
     """(logp f32 [...], lse f32 [...]): log-probability of the given labels and the rows' log-sum-exp.  logits f32 / bf16 [..., ldl], labels
     int64 [...]; a label outside [0, num_classes) has logp 0."""
-    dt, ldl, M = _rows(logits, labels, num_classes)
-    with _on(logits):
-        logp = torch.empty(labels.shape, dtype=torch.float32, device=logits.device)
-        lse = torch.empty_like(logp)
-        ws = _scratch(_lib.load().emadapt_label_logp_workspace_bytes(M, int(num_classes)), logits)
-        _lib.call("emadapt_label_logp", _p(logits), dt, ldl, _p(labels), M, int(num_classes), _p(logp), _p(lse), _p(ws),
-                  0 if ws is None else ws.numel(), _stream())
+    dt, ldl, M, C = _rows(logits, labels, num_classes)
+    logp, lse = _f32(labels.shape, logits), _f32(labels.shape, logits)
+    _launch(logits, "emadapt_label_logp", logits.data_ptr(), dt, ldl, labels.data_ptr(), M, C, logp.data_ptr(), lse.data_ptr())
     return logp, lse
 
 
 def label_logp_bwd(logits, labels, lse, dlogp, num_classes, dlogits=None):
     """d loss / d logits from d loss / d logp and the lse of label_logp: ([c = label] - softmax) * dlogp, 0 in rows without a label and in the
     padding columns.  dlogits: f32 / bf16 output of the logits' shape (default: their type); it must not overlap the logits."""
-    dt, ldl, M = _rows(logits, labels, num_classes)
-    _row_vector(lse, logits, M, "lse")
-    _row_vector(dlogp, logits, M, "dlogp")
-    with _on(logits):
-        dlogits, ddt = _dlogits(logits, dlogits)
-        _lib.call("emadapt_label_logp_bwd", _p(logits), dt, ldl, _p(labels), _p(lse), _p(dlogp), M, int(num_classes), _p(dlogits), ddt, _stream())
+    dt, ldl, M, C = _rows(logits, labels, num_classes)
+    if lse is None or dlogp is None:
+        raise ValueError("lse and dlogp are needed")
+    lse, dlogp = _row_vector(lse, logits, M, "lse"), _row_vector(dlogp, logits, M, "dlogp")
+    dlogits, ddt = _dlogits(logits, dt, dlogits)
+    _launch(logits, "emadapt_label_logp_bwd", logits.data_ptr(), dt, ldl, labels.data_ptr(), lse, dlogp, M, C, dlogits.data_ptr(), ddt)
     return dlogits
 
 
@@ -924,27 +934,25 @@ def policy_loss(logits, actions, old_logp, advantages, num_classes, ref_logp=Non
     old_logp, advantages, ref_logp, weights: f32 [...] (the last two optional).  Returns (sums f32 [4], logp f32 [...], dlogits or None); sums =
     weighted sums over the rows of the loss, its surrogate part, its KL part, and the rows whose ratio the clip holds; dlogits = grad_scale (default
     1 / rows) times the gradient of sums[0]."""
-    dt, ldl, M = _rows(logits, actions, num_classes, "actions")
-    for t, name in ((old_logp, "old_logp"), (advantages, "advantages"), (ref_logp, "ref_logp"), (weights, "weights")):
-        _row_vector(t, logits, M, name)
+    dt, ldl, M, C = _rows(logits, actions, num_classes, "actions")
     if old_logp is None or advantages is None:
         raise ValueError("old_logp and advantages are needed")
+    old, adv = _row_vector(old_logp, logits, M, "old_logp"), _row_vector(advantages, logits, M, "advantages")
+    ref, weight = _row_vector(ref_logp, logits, M, "ref_logp"), _row_vector(weights, logits, M, "weights")
     if not 0.0 <= clip_low <= 1.0 or not clip_high >= 0.0:
         raise ValueError("clip_low must be in [0, 1] and clip_high >= 0, got %r and %r" % (clip_low, clip_high))
-    if ref_logp is None and kl_coef != 0.0:
+    if ref is None and kl_coef != 0.0 and M:
         raise ValueError("a KL term needs ref_logp")
     if grad_scale is None:
         grad_scale = 1.0 / max(M, 1)
-    with _on(logits):
-        ddt = DT_F32
-        if want_grad:
-            dlogits, ddt = _dlogits(logits, dlogits)
-        sums = torch.empty(4, dtype=torch.float32, device=logits.device)
-        logp = torch.empty(actions.shape, dtype=torch.float32, device=logits.device)
-        ws = _scratch(_lib.load().emadapt_policy_loss_workspace_bytes(M, int(num_classes)), logits)
-        _lib.call("emadapt_policy_loss", _p(logits), dt, ldl, _p(actions), _p(old_logp), _p(ref_logp), _p(advantages), _p(weights), M, int(num_classes),
-                  float(clip_low), float(clip_high), float(kl_coef), float(grad_scale), _p(sums), _p(logp), _p(dlogits) if want_grad else None, ddt,
-                  _p(ws), ws.numel(), _stream())
+    ddt = DT_F32
+    if want_grad:
+        dlogits, ddt = _dlogits(logits, dt, dlogits)
+    sums, logp = _f32(4, logits), _f32(actions.shape, logits)
+    nbytes = _lib.load().emadapt_policy_loss_workspace_bytes(M, C)
+    ws = _scratch(nbytes, logits)
+    _launch(logits, "emadapt_policy_loss", logits.data_ptr(), dt, ldl, actions.data_ptr(), old, ref, adv, weight, M, C, clip_low, clip_high, kl_coef,
+            grad_scale, sums.data_ptr(), logp.data_ptr(), dlogits.data_ptr() if want_grad else None, ddt, ws.data_ptr(), nbytes)
     return sums, logp, (dlogits if want_grad else None)
 
 
@@ -954,7 +962,9 @@ def preference_loss(logits, labels, seq_start, ref_logp, num_classes, beta=0.1, 
     [2 * pairs] the reference model's sequence log-probabilities.
 
     Returns (loss f32 [pairs], seq_logp f32 [2 * pairs], dlogits or None); dlogits = grad_scale (default 1 / pairs) times the gradient of loss.sum()."""
-    dt, ldl, M = _rows(logits, labels, num_classes)
+    dt, ldl, M, C = _rows(logits, labels, num_classes)
+    if seq_start is None or ref_logp is None:
+        raise ValueError("seq_start and ref_logp are needed")
     _check(seq_start, torch.int64, "seq_start")
     _same_device(logits, seq_start, "seq_start")
     if seq_start.dim() != 1 or seq_start.numel() % 2 != 1:
@@ -968,16 +978,14 @@ def preference_loss(logits, labels, seq_start, ref_logp, num_classes, beta=0.1, 
         raise ValueError("label_smoothing must be in [0, 1], got %r" % label_smoothing)
     if grad_scale is None:
         grad_scale = 1.0 / max(pairs, 1)
-    with _on(logits):
-        ddt = DT_F32
-        if want_grad:
-            dlogits, ddt = _dlogits(logits, dlogits)
-        loss = torch.empty(pairs, dtype=torch.float32, device=logits.device)
-        seq_logp = torch.empty(2 * pairs, dtype=torch.float32, device=logits.device)
-        ws = _scratch(_lib.load().emadapt_preference_loss_workspace_bytes(M, int(num_classes)), logits)
-        _lib.call("emadapt_preference_loss", _p(logits), dt, ldl, _p(labels), _p(seq_start), pairs, _p(ref_logp), M, int(num_classes), float(beta),
-                  float(label_smoothing), float(grad_scale), _p(loss), _p(seq_logp), _p(dlogits) if want_grad else None, ddt, _p(ws),
-                  0 if ws is None else ws.numel(), _stream())
+    ddt = DT_F32
+    if want_grad:
+        dlogits, ddt = _dlogits(logits, dt, dlogits)
+    loss, seq_logp = _f32(pairs, logits), _f32(2 * pairs, logits)
+    nbytes = _lib.load().emadapt_preference_loss_workspace_bytes(M, C)
+    ws = _scratch(nbytes, logits)
+    _launch(logits, "emadapt_preference_loss", logits.data_ptr(), dt, ldl, labels.data_ptr(), seq_start.data_ptr(), pairs, ref_logp.data_ptr(), M, C, beta,
+            label_smoothing, grad_scale, loss.data_ptr(), seq_logp.data_ptr(), dlogits.data_ptr() if want_grad else None, ddt, ws.data_ptr(), nbytes)
     return loss, seq_logp, (dlogits if want_grad else None)
 
 
@@ -1031,7 +1039,7 @@ class AdamW:
         self._control = torch.zeros(lib.emadapt_adamw_control_bytes(), dtype=torch.uint8, device=self.device)
         self.steps = self._control[:8].view(torch.int64)
         self.grad_norm = self._control[8:12].view(torch.float32)
-        self._step = lib.emadapt_adamw_step
+        self._control_bytes = self._control.numel()
         self.set_grads(grads)
 
     def set_grads(self, grads):
@@ -1063,8 +1071,7 @@ class AdamW:
         _lib.call("emadapt_adamw_table", len(grads), arr, dt, ADAMW_STATES[self.state], ctypes.c_void_p(host.data_ptr()), host.numel())
         self.grads, self._gdt, self._chunks = grads, dt, chunks
         self._grads_apart = None
-        with _on(self._control):
-            self._table = host.to(self.device)
+        self._table = host.to(self.device)
 
     def step(self, lr, grad_scale=1.0, max_norm=0.0, zero_grads=False):
         """One step: gradients times grad_scale, held to the global norm max_norm (0: not), weights and moments updated in place.  zero_grads: the
@@ -1073,12 +1080,8 @@ class AdamW:
         if zero_grads and not self._grads_apart:
             _refuse_overlap(self.grads, "grads")
             self._grads_apart = True
-        with _on(self._control):
-            rc = self._step(self._table.data_ptr(), self._chunks, self._gdt, ADAMW_STATES[self.state], self._control.data_ptr(), self._control.numel(),
-                            float(lr), self.betas[0], self.betas[1], self.eps, float(grad_scale), float(max_norm), self.seed, 1 if zero_grads else 0,
-                            torch.cuda.current_stream().cuda_stream)
-        if rc:
-            raise _lib.EmadaptError(rc, "emadapt_adamw_step")
+        _launch(self._control, "emadapt_adamw_step", self._table.data_ptr(), self._chunks, self._gdt, ADAMW_STATES[self.state], self._control.data_ptr(),
+                self._control_bytes, lr, self.betas[0], self.betas[1], self.eps, grad_scale, max_norm, self.seed, 1 if zero_grads else 0)
 
     def unpack(self, dtype=torch.float32):
         """(m, u) of the 8-bit states as flat tensors of values (exact in float32 and bfloat16); u is the root of the second moment."""
@@ -1086,11 +1089,10 @@ class AdamW:
             raise ValueError("unpack() is for 8-bit states; m and v of 32-bit states are there as they are")
         if dtype not in (torch.float32, torch.bfloat16):
             raise TypeError("states unpack to float32 or bfloat16, got %s" % dtype)
-        with _on(self._control):
-            m = torch.empty(self.total, dtype=dtype, device=self.device)
-            u = torch.empty(self.total, dtype=dtype, device=self.device)
-            _lib.call("emadapt_adamw_unpack", _p(self.m8), _p(self.u8), _p(self.powers), self.total, _p(m), _p(u),
-                      DT_BF16 if dtype == torch.bfloat16 else DT_F32, _stream())
+        m = torch.empty(self.total, dtype=dtype, device=self.device)
+        u = torch.empty(self.total, dtype=dtype, device=self.device)
+        _launch(m, "emadapt_adamw_unpack", self.m8.data_ptr(), self.u8.data_ptr(), self.powers.data_ptr(), self.total, m.data_ptr(), u.data_ptr(),
+                _DT_OF[dtype])
         return m, u
 
     def pack(self, m, u):
@@ -1101,8 +1103,7 @@ class AdamW:
             _check(t, name=name)
             if t.numel() != self.total or t.device != self.device:
                 raise ValueError("%s must hold the %d elements of the state buffers on %s" % (name, self.total, self.device))
-        with _on(self._control):
-            _lib.call("emadapt_adamw_pack", _p(m), _p(u), self.total, _p(self.m8), _p(self.u8), _p(self.powers), _stream())
+        _launch(self._control, "emadapt_adamw_pack", m.data_ptr(), u.data_ptr(), self.total, self.m8.data_ptr(), self.u8.data_ptr(), self.powers.data_ptr())
 
 
 def _per_tensor(v, n, name):

@@ -555,9 +555,8 @@ int emadapt_sgd_accumulate_pack(const float *g, const float *w, int64_t n, int64
  * ---------------------------------------------------------------------------------------- */
 
 /* lse[r] = log sum_{c < C} exp(logits[r][c]);  logp[r] = logits[r][labels[r]] - lse[r].  Either output may be NULL. */
-size_t emadapt_label_logp_workspace_bytes(int64_t M, int64_t C);
 int emadapt_label_logp(const void *logits, int dtype, int64_t ldl, const int64_t *labels, int64_t M, int64_t C, float *logp, float *lse,
-                       void *workspace, size_t workspace_bytes, void *stream);
+                       void *stream);
 /* dlogits[r][c] = ([c == labels[r]] - exp(logits[r][c] - lse[r])) * dlogp[r]; a row with dlogp 0 is 0. */
 int emadapt_label_logp_bwd(const void *logits, int dtype, int64_t ldl, const int64_t *labels, const float *lse, const float *dlogp,
                            int64_t M, int64_t C, void *dlogits, int dlogits_dtype, void *stream);

@@ -14,8 +14,8 @@ def lib():
     return _lib.load()
 
 
-def _logp(lib, logits=4096, dtype=0, ldl=24, labels=8192, M=4, C=21, logp=16384, lse=None, ws=None, nws=0):
-    return lib.emadapt_label_logp(logits, dtype, ldl, labels, M, C, logp, lse, ws, nws, None)
+def _logp(lib, logits=4096, dtype=0, ldl=24, labels=8192, M=4, C=21, logp=16384, lse=None):
+    return lib.emadapt_label_logp(logits, dtype, ldl, labels, M, C, logp, lse, None)
 
 
 @pytest.mark.parametrize("kw", [dict(dtype=2), dict(M=-1), dict(C=0), dict(ldl=20), dict(logits=None), dict(labels=None), dict(labels=8196),
