@@ -89,6 +89,13 @@ class ADAPT(Network):
         self._step = 0
         self._micro = 0
         self._estep_cfg = None
+        # "momentum" (the reference's), "adamw" or "adamw8" (ops.AdamW with 32- / 8-bit moments over the 32 tensors; config "betas",
+        # "adam_eps", "max_grad_norm").  The weight decay of pre_train() is then decoupled, and on the filters alone as before.
+        self.optimizer = str(self.config.get("optimizer", "momentum"))
+        if self.optimizer not in ("momentum", "adamw", "adamw8"):
+            raise ValueError("optimizer must be 'momentum', 'adamw' or 'adamw8', got %r" % self.optimizer)
+        self._adamw = None
+        self._adamw_source = None
         self._weight_decay = 0.0
         self._momentum = 0.9
         self._gradsync = None
@@ -638,6 +645,16 @@ class ADAPT(Network):
     def optimize(self, base_lr, momentum):
         self.net["lr"] = float(base_lr)
         self._momentum = float(momentum)
+        if self.optimizer != "momentum":
+            params, decay = [], []
+            for layer in self._segments:
+                s, nw, nb = (self._segments[layer][k] for k in ("start", "nw", "nb"))
+                params += [self._flat["params"][s:s + nw], self._flat["params"][s + nw:s + nw + nb]]
+                decay += [self._weight_decay, 0.0]
+            self._adamw = ops.AdamW(params, self._adamw_grads(self._flat["accum"]), state="u8" if self.optimizer == "adamw8" else "f32",
+                                    betas=tuple(self.config.get("betas", (0.9, 0.999))), eps=float(self.config.get("adam_eps", 1e-8)),
+                                    weight_decay=decay, seed=self.seed)
+            self._adamw_source = self._flat["accum"]
         # the three "ops" of the reference's loop (deeplab.py:202-205), as callables
         self.net["accum_gradient"] = self._flat["accum"]
         self.net["accum_gradient_accum"] = self.micro_step
@@ -672,6 +689,32 @@ class ADAPT(Network):
             # and raises its own word (include/emadapt.h, emadapt_status_collective)
             ops.status_collective(True)
 
+    def _adamw_grads(self, flat):
+        """The 32 tensors' gradients in a buffer laid out like the flat parameters (accumulators, one micro-batch's gradients, the exchange's payload)."""
+        got = []
+        for seg in self._segments.values():
+            s, nw, nb = seg["start"], seg["nw"], seg["nb"]
+            got += [flat[s:s + nw], flat[s + nw:s + nw + nb]]
+        return got
+
+    def _adamw_update(self, scale):
+        """apply_update() with AdamW: the gradients are read where the mode leaves them, the accumulators zeroed (the clean op)."""
+        f, gs = self._flat, self._gradsync
+        clean = False
+        if self._pending_fused:
+            source, scale = f["grads"], scale / float(self.accum_num)
+            self._pending_fused = False
+        elif gs is not None and not gs.writeback:
+            source = gs.gathered
+            if not gs.prepacked:
+                f["accum"].zero_()
+        else:
+            source, clean = f["accum"], True
+        if source is not self._adamw_source:
+            self._adamw.set_grads(self._adamw_grads(source))
+            self._adamw_source = source
+        self._adamw.step(self.net["lr"], grad_scale=scale, max_norm=float(self.config.get("max_grad_norm", 0.0)), zero_grads=clean)
+
     def _bucket_order(self):
         return [self._segments[op.name] for op in reversed(self._plan) if op.kind == "conv"]
 
@@ -693,6 +736,7 @@ class ADAPT(Network):
         d = dlogits
         cur, other = bufs["gA"], bufs["gB"]
         inv_accum = 1.0 / float(self.accum_num)
+        decay = self._weight_decay if self._adamw is None else 0.0   # (AdamW's decay is not a part of the gradient)
         plan = self._plan
         bf16 = self.compute_dtype == "bf16"
         x6 = self.compute_dtype == "bf16x6"
@@ -733,11 +777,11 @@ class ADAPT(Network):
                 seg = op.seg
                 s, n = seg["start"], seg["nw"] + seg["nb"]
                 if sync is not None and sync.prepacked:
-                    ops.sgd_accumulate_pack(self._flat["grads"][s:s + n], self._flat["params"][s:s + n], seg["nw"], self._weight_decay,
+                    ops.sgd_accumulate_pack(self._flat["grads"][s:s + n], self._flat["params"][s:s + n], seg["nw"], decay,
                                             inv_accum, out=sync.sendfull[s:s + n])
                 elif not fused:
                     ops.sgd_accumulate(self._flat["accum"][s:s + n], self._flat["grads"][s:s + n],
-                                       self._flat["params"][s:s + n], seg["nw"], self._weight_decay, inv_accum)
+                                       self._flat["params"][s:s + n], seg["nw"], decay, inv_accum)
                 if last_micro and self._gradsync is not None:
                     self._gradsync.segment_ready(seg["start"], seg["end"])
                 if prev is None:
@@ -778,6 +822,53 @@ class ADAPT(Network):
         self._micro += 1
         return self.loss["norm"]
 
+    # -- training on rewards and preferences (beside micro_step: the same forward, backward and update) -----------------------
+    def _own_loss(self, images, keep_prob, loss):
+        """One micro-batch with a loss of its own over the logits: loss(logits, dlogits) fills dlogits."""
+        self.forward(images, keep_prob, for_backward=True)
+        logits = self._bufs["act"][self._plan[-1].name]
+        dl = self._bufs["gA"][:logits.numel()].view(logits.shape)
+        out = loss(logits, dl)
+        self.backward(dl, last_micro=(self._micro % self.accum_num) == self.accum_num - 1)
+        self._micro += 1
+        return out
+
+    def label_logp(self, images, labels, keep_prob=1.0):
+        """Log-probability f32 [B,S,S] of the label maps int64 [B,S,S] (S = the logits' size, 255 = void: 0) under the network as it is: what
+        policy_step takes as old_logp / ref_logp."""
+        self.forward(images, keep_prob)
+        return ops.label_logp(self._bufs["act"][self._plan[-1].name], self._to_dev(labels, torch.int64), self.category_num)[0]
+
+    def policy_step(self, images, labels, old_logp, advantages, ref_logp=None, weights=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, keep_prob=1.0):
+        """One micro-batch of the clipped policy loss (ops.policy_loss, mean over the pixels) on sampled label maps int64 [B,S,S]: forward, loss, backward,
+        accumulate.  advantages (and weights): f32 [B,S,S], or one per image [B].  Returns (sums, logp)."""
+        lab = self._to_dev(labels, torch.int64)
+
+        def rows(v):
+            if v is None:
+                return None
+            v = self._to_dev(v)
+            return v.view(-1, 1, 1).expand(lab.shape).contiguous() if v.dim() == 1 else v
+
+        old, adv, ref, w = (rows(v) for v in (old_logp, advantages, ref_logp, weights))
+        sums, logp = self._own_loss(images, keep_prob, lambda z, dl: ops.policy_loss(
+            z, lab, old, adv, self.category_num, ref_logp=ref, weights=w, clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef, dlogits=dl)[:2])
+        self.loss["norm"] = sums[:1] / max(lab.numel(), 1)
+        return sums, logp
+
+    def preference_step(self, images, labels, ref_logp, beta=0.1, label_smoothing=0.0, keep_prob=1.0):
+        """One micro-batch of the preference loss (ops.preference_loss, mean over the pairs): images [2P,H,W,3] with label maps int64 [2P,S,S], entry 2j
+        preferred to entry 2j + 1; ref_logp f32 [2P]: the maps' summed log-probabilities under the reference network.  Returns (loss [P], map_logp [2P])."""
+        lab = self._to_dev(labels, torch.int64)
+        if lab.shape[0] % 2:
+            raise ValueError("preference_step takes pairs: %d label maps" % lab.shape[0])
+        at = torch.arange(lab.shape[0] + 1, device=self.device) * (lab.numel() // max(lab.shape[0], 1))
+        ref = self._to_dev(ref_logp)
+        loss, seq = self._own_loss(images, keep_prob, lambda z, dl: ops.preference_loss(z, lab, at, ref, self.category_num, beta=beta,
+                                                                                      label_smoothing=label_smoothing, dlogits=dl)[:2])
+        self.loss["norm"] = loss.mean()
+        return loss, seq
+
     def apply_update(self):
         """accum_gradient_update + accum_gradient_clean (deeplab.py:203-205,268-270)."""
         scale = 1.0
@@ -787,7 +878,9 @@ class ADAPT(Network):
             gs.wait()
             scale = 1.0 / gs.world_size
         fresh = set()
-        if self._pending_fused:
+        if self._adamw is not None:
+            self._adamw_update(scale)
+        elif self._pending_fused:
             tiles = self.compute_dtype == "bf16" and self.config.get("fused_tiles", True)
             rest = []   # (start, n, n_decay) of the layers without a pass of their own: one launch for all of them
             for op in self._plan:   # accumulate + apply_gradients + clean of the one micro-batch

@@ -154,6 +154,20 @@ class _Saver:
         v = n._flat["momentum"]
         return v[s:s + nw].view(seg["pshape"])[:, :, :cin, :cout], v[s + nw:s + nw + nb][:cout]
 
+    def _adamw_slots(self, m, v):
+        """{layer: (m of the filter, m of the bias, v of the filter, v of the bias)}: views of the flat state values in the layers' unpadded shapes."""
+        n, got = self.netobj, {}
+        for k, layer in enumerate(n._segments):
+            seg = n._segments[layer]
+            kh, kw, cin, cout = seg["shape"]
+            a, b = n._adamw.offsets[2 * k], n._adamw.offsets[2 * k + 1]
+            got[layer] = tuple(x for t in (m, v) for x in (t[a:a + seg["nw"]].view(seg["pshape"])[:, :, :cin, :cout], t[b:b + seg["nb"]][:cout]))
+        return got
+
+    def _adamw_values(self):
+        o = self.netobj._adamw
+        return (o.m, o.v) if o.state == "f32" else o.unpack()
+
     def save(self, sess, path, global_step=None):
         n = self.netobj
         if global_step is not None:
@@ -166,10 +180,16 @@ class _Saver:
         for layer, (w, b) in n.weights.items():
             blob[layer + "_weights"] = w.detach().cpu().numpy()
             blob[layer + "_bias"] = b.detach().cpu().numpy()
-            if getattr(n, "_flat", None) is not None:
+            if getattr(n, "_flat", None) is not None and getattr(n, "_adamw", None) is None:
                 vw, vb = self._momentum_views(layer)
                 blob[layer + "_weights/Momentum"] = vw.detach().cpu().numpy()
                 blob[layer + "_bias/Momentum"] = vb.detach().cpu().numpy()
+        if getattr(n, "_adamw", None) is not None:   # (second: v, or the 8-bit states' root of v)
+            for layer, slots in self._adamw_slots(*self._adamw_values()).items():
+                for name, t in zip(("_weights/Adam", "_bias/Adam", "_weights/Adam_1", "_bias/Adam_1"), slots):
+                    blob[layer + name] = t.detach().cpu().numpy()
+            blob["adam_steps"] = n._adamw.steps.cpu().numpy()
+            blob["adam_state"] = np.array(n._adamw.state)
         tmp = "%s.tmp.%d" % (final, os.getpid())
         with open(tmp, "wb") as f:
             np.savez(f, **blob)
@@ -197,6 +217,7 @@ class _Saver:
         if not path.endswith(".npz"):
             path = path + ".npz"
         flat = getattr(n, "_flat", None)
+        adamw = getattr(n, "_adamw", None)
         with np.load(path) as z:
             slots = 0
             for layer, (w, b) in n.weights.items():
@@ -207,7 +228,18 @@ class _Saver:
                     vw.copy_(torch.from_numpy(z[layer + "_weights/Momentum"]).to(vw.device))
                     vb.copy_(torch.from_numpy(z[layer + "_bias/Momentum"]).to(vb.device))
                     slots += 1
-            if flat is not None and slots == 0:
+            if adamw is not None:
+                if "adam_state" in z.files and str(z["adam_state"]) == adamw.state:
+                    m, v = self._adamw_values()
+                    for layer, views in self._adamw_slots(m, v).items():
+                        for name, t in zip(("_weights/Adam", "_bias/Adam", "_weights/Adam_1", "_bias/Adam_1"), views):
+                            t.copy_(torch.from_numpy(z[layer + name]).to(t.device))
+                    if adamw.state == "u8":
+                        adamw.pack(m, v)
+                    adamw.steps.copy_(torch.from_numpy(z["adam_steps"]).to(adamw.device))
+                else:
+                    warnings.warn("checkpoint %s holds no %s moments of AdamW -- weights restored, the moments left as they are" % (path, adamw.state))
+            elif flat is not None and slots == 0:
                 # round-1 files hold the whole (padded) momentum buffer as one array: usable when the layout still matches
                 if _LEGACY_MOMENTUM in z.files and z[_LEGACY_MOMENTUM].size == flat["momentum"].numel():
                     flat["momentum"].copy_(torch.from_numpy(z[_LEGACY_MOMENTUM]).reshape(-1).to(flat["momentum"].device))
