@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(256) adamw_norm_kernel(const AdamwChunk *__res
     if (threadIdx.x == 0) {
         __hip_atomic_store(&ctl->sum[blockIdx.x], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __builtin_amdgcn_s_waitcnt(0);
-        last = __hip_atomic_fetch_add(&ctl->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        last = atomicInc(&ctl->ticket, gridDim.x - 1) == gridDim.x - 1;   // (back to 0 by itself)
     }
     __syncthreads();
     if (!last) return;
@@ -153,7 +153,6 @@ __global__ void __launch_bounds__(256) adamw_norm_kernel(const AdamwChunk *__res
     for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) s += __hip_atomic_load(&ctl->sum[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     s = block_sum_f64(s, sh);
     if (threadIdx.x != 0) return;
-    ctl->ticket = 0u;
     adamw_control(ctl, a, s, status);
 }
 
@@ -381,7 +380,12 @@ __global__ void __launch_bounds__(256) adamw_pack_kernel(const float *__restrict
         float mv[4], uv[4], mtop = 0.f, utop = 0.f;
         load4((const EMADAPT_GLOBAL float *)m + q * 4, mv); load4((const EMADAPT_GLOBAL float *)u + q * 4, uv);
 #pragma unroll
-        for (int k = 0; k < 4; k++) { mv[k] = fminf(fmaxf(mv[k], -kMostM), kMostM); uv[k] = fminf(fmaxf(uv[k], 0.f), kMostU); mtop = fmaxf(mtop, fabsf(mv[k])); utop = fmaxf(utop, uv[k]); }
+        for (int k = 0; k < 4; k++) {   // (NaN: 0)
+            mv[k] = mv[k] == mv[k] ? fminf(fmaxf(mv[k], -kMostM), kMostM) : 0.f;
+            uv[k] = fminf(fmaxf(uv[k], 0.f), kMostU);
+            mtop = fmaxf(mtop, fabsf(mv[k]));
+            utop = fmaxf(utop, uv[k]);
+        }
         const int em = block_power<3>(row_top(mtop)), eu = block_power<4>(row_top(utop));
         unsigned mo = 0, uo = 0;
 #pragma unroll
@@ -427,6 +431,7 @@ int emadapt_adamw_table(int count, const emadapt_adamw_tensor *tensors, int grad
         const emadapt_adamw_tensor &t = tensors[k];
         if (t.n == 0) continue;
         if (!t.w || !t.g || !t.m || !t.v || !aligned(t.w, 4) || !aligned(t.g, gs) || t.unit < 0 || t.unit % 4) return EMADAPT_ERR_INVALID;
+        if (!isfinite(t.weight_decay) || !isfinite(t.lr_scale)) return EMADAPT_ERR_INVALID;
         // (codes are read four at a time and the powers of two by pairs; f32 moments at their own alignment)
         if (state == EMADAPT_ADAMW_U8 ? (!t.e || !aligned(t.m, 4) || !aligned(t.v, 4) || !aligned(t.e, 2)) : (!aligned(t.m, 4) || !aligned(t.v, 4)))
             return EMADAPT_ERR_INVALID;
@@ -451,7 +456,8 @@ int emadapt_adamw_table(int count, const emadapt_adamw_tensor *tensors, int grad
 int emadapt_adamw_step(const void *table, int64_t chunks, int grad_dtype, int state, void *control, size_t control_bytes, double lr, double beta1,
                        double beta2, double eps, float grad_scale, double max_norm, unsigned seed, int zero_grads, void *stream_) {
     if (!is_dt(grad_dtype) || (state != EMADAPT_ADAMW_F32 && state != EMADAPT_ADAMW_U8)) return EMADAPT_ERR_INVALID;
-    if (chunks < 0 || (chunks && !table) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 1e-16) || !(max_norm >= 0.0))
+    if (chunks < 0 || (chunks && !table) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 1e-16) || !(max_norm >= 0.0) ||
+        !isfinite(lr) || !isfinite(grad_scale))
         return EMADAPT_ERR_INVALID;
     if (!control || control_bytes < sizeof(AdamwControl)) return EMADAPT_ERR_WORKSPACE;
     if (chunks > 0x7FFFFFFF / kRounds) return EMADAPT_ERR_UNSUPPORTED;

@@ -122,8 +122,34 @@ struct Rows {
     bool last;   // nor are the logits, which are read for the last time
 };
 
-// dz = [c = label] coef - exp(z - base) coef / sum (base, sum: the row's maximum and sum; without sum the log-sum-exp): every thread kUnroll vectors of the flattened [M][vectors per row], all in flight.  A
-// workgroup's vectors lie behind one another; their rows come from one 64-bit division for the workgroup and a 32-bit one for each vector.
+// An f32 log-sum-exp of this size and more keeps too little of the sum (2^-12 of a probability is rounding here, and of a row masked as a whole with
+// the type's lowest value the log C is gone): one wave takes the rows' maxima and sums anew, one row after the other, for its lanes.  A lane whose
+// lse is not the one of its row (a part of the classes, say) keeps it.
+constexpr float kFar = 4096.f;
+template <typename T>
+__device__ void sums_anew(const Rows &a, long long row, bool far, float f, float &base, float &fs) {
+    for (unsigned long long left = __ballot(far); left;) {
+        const long long r = __shfl(row, __ffsll((long long)left) - 1);
+        const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
+        float m = -INFINITY, s = 0.f;
+#pragma unroll 1
+        for (int i = threadIdx.x & 63; i < a.C; i += 64) m = fmaxf(m, (float)z[i]);
+        m = group_max<64>(m);
+#pragma unroll 1
+        for (int i = threadIdx.x & 63; i < a.C; i += 64) s += __expf((float)z[i] - m);
+        s = group_sum<64>(s);
+        const bool mine = far && row == r;
+        if (mine && fabsf(m + logf(s) - base) <= 0x1p-22f * fabsf(base)) {
+            base = m;
+            fs = f / s;
+        }
+        left &= ~__ballot(mine);
+    }
+}
+
+// dz = [c = label] coef - exp(z - base) coef / sum (base, sum: the row's maximum and sum; without sum the log-sum-exp): every thread kUnroll vectors
+// of the flattened [M][vectors per row], all in flight.  A workgroup's vectors lie behind one another; their rows come from one 64-bit division for
+// the workgroup and a 32-bit one for each vector.
 template <typename T, typename TD, int kUnroll>
 __global__ void __launch_bounds__(256) row_grad_kernel(Rows a, const float *__restrict__ base, const float *__restrict__ sum, const float *__restrict__ coef, TD *__restrict__ dlogits,
                                                       unsigned nvec, long long total) {
@@ -148,6 +174,13 @@ __global__ void __launch_bounds__(256) row_grad_kernel(Rows a, const float *__re
         l[q] = base[row[q]];
         f[q] = used ? coef[row[q]] : 0.f;
         fs[q] = sum ? f[q] * __builtin_amdgcn_rcpf(sum[row[q]]) : f[q];
+    }
+    if (!sum) {
+#pragma unroll
+        for (int q = 0; q < kUnroll; q++) {
+            const bool far = row[q] >= 0 && f[q] != 0.f && fabsf(l[q]) >= kFar && fabsf(l[q]) < INFINITY;
+            if (__any(far)) sums_anew<T>(a, row[q], far, f[q], l[q], fs[q]);
+        }
     }
 #pragma unroll
     for (int q = 0; q < kUnroll; q++) {
@@ -191,12 +224,12 @@ __device__ __forceinline__ float policy_row(float log_ratio, float q, bool has_r
         const float k = !has_ref ? 0.f
                         : fabsf(q) < 0.5f ? q * q * (1.f / 2 + q * (1.f / 6 + q * (1.f / 24 + q * (1.f / 120 + q * (1.f / 720 + q * (1.f / 5040 + q * (1.f / 40320)))))))
                                           : e - q;
-        t.loss += (double)w * (double)(part + p.kl * k);
+        t.loss += (double)w * (double)(p.kl != 0.f ? part + p.kl * k : part);
         t.surrogate += (double)w * (double)part;
         t.kl += (double)w * (double)k;
         t.clipped += clipped ? (double)w : 0.0;
     }
-    return w * p.scale * ((clipped ? 0.f : free) - p.kl * e);
+    return w * p.scale * ((clipped ? 0.f : free) - (p.kl != 0.f ? p.kl * e : 0.f));   // (e may have overflowed: no term, not 0 * inf)
 }
 // is the log of the ratio past the border that its advantage's sign puts up?
 __device__ __forceinline__ bool past_border(double log_ratio, float adv, const Policy &p) {
@@ -210,15 +243,15 @@ __device__ __forceinline__ bool near_border(double log_ratio, float adv, const P
     const double border = adv > 0.f ? p.log_high : p.log_low;
     return adv != 0.f && fabs(log_ratio - border) < (double)p.tol;
 }
-// sum over elements `first`, first + step, .. of the row of exp(z - z_label) in 64 bits
+// sum over elements `first`, first + step, .. of the row of exp(z - its maximum) in 64 bits; the label's log-probability from the whole sum
 template <typename T>
-__device__ double exact_part(const T *z, int C, long long lab, int first, int step) {
-    const double at = (double)(float)z[lab];
+__device__ double exact_part(const T *z, int C, float top, int first, int step) {
     double s = 0.0;
 #pragma unroll 1
-    for (int i = first; i < C; i += step) s += exp((double)(float)z[i] - at);
+    for (int i = first; i < C; i += step) s += exp((double)(float)z[i] - (double)top);
     return s;
 }
+__device__ __forceinline__ double exact_logp(float z, float top, double sum) { return ((double)z - (double)top) - log(sum); }
 
 // ------------------------------------------------------------------------------------------
 // rows that stay in registers: one pass over the logits
@@ -311,9 +344,9 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
                 bool near;
                 f = policy_of_row(p, x, zl, MaxSum{m, s}, lane == 0, lp, near, t);
                 if (near) {
-                    double e = exact_part(z, a.C, lab, lane, L);
+                    double e = exact_part(z, a.C, m, lane, L);
                     for (int o = L / 2; o > 0; o >>= 1) e += __shfl_xor(e, o);
-                    f = policy_of_exact(p, x, -log(e), lane == 0, lp, t);
+                    f = policy_of_exact(p, x, exact_logp(zl, m, e), lane == 0, lp, t);
                 }
             }
         }
@@ -535,7 +568,9 @@ __global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const
         for (int q = 0; q < 4; q++)
             for (unsigned long long left = mask[q]; left; left &= left - 1) {
                 const long long rr = r0 + q * 64 + (__ffsll((long long)left) - 1);
-                const double lp64 = -log(block_sum_f64(exact_part(static_cast<const T *>(a.logits) + rr * a.ldl, a.C, a.labels[rr], threadIdx.x, 256), sh));
+                const T *z = static_cast<const T *>(a.logits) + rr * a.ldl;
+                const float top = base[rr];
+                const double lp64 = exact_logp((float)z[a.labels[rr]], top, block_sum_f64(exact_part(z, a.C, top, threadIdx.x, 256), sh));
                 if (threadIdx.x == 0) {
                     float lp;
                     coef[rr] = policy_of_exact(p, policy_inputs(p, rr), lp64, true, lp, t);
@@ -560,6 +595,7 @@ template <typename T, typename TD>
 __global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, Outputs out, int nparts, double *__restrict__ fixed, float *__restrict__ sums) {
     __shared__ double sh[16][4];
     __shared__ double one[16];
+    __shared__ MaxSum pair[16];
     __shared__ unsigned long long mask[16];
     __shared__ bool last;
     PolicyTerms t = {0, 0, 0, 0};
@@ -572,15 +608,20 @@ __global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, O
             for (unsigned long long left = mask[q]; left; left &= left - 1) {
                 const long long r = r0 + q * 64 + (__ffsll((long long)left) - 1), lab = a.labels[r];
                 const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
-                const double lp64 = -log(block_sum_f64(exact_part(z, a.C, lab, threadIdx.x, 1024), one));
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int i = threadIdx.x; i < a.C; i += 1024) top = fmaxf(top, (float)z[i]);
+                top = block_join<16>(MaxSum{group_max<64>(top), 0.f}, pair).m;
+                const double sum = block_sum_f64(exact_part(z, a.C, top, threadIdx.x, 1024), one), lp64 = exact_logp((float)z[lab], top, sum);
                 float lp;
                 const float f = policy_of_exact(p, policy_inputs(p, r), lp64, threadIdx.x == 0, lp, t);
                 if (threadIdx.x == 0) out.logp[r] = lp;
                 if (!out.dlogits) continue;
-                const float lse = (float)((double)(float)z[lab] - lp64);
                 TD *d = static_cast<TD *>(out.dlogits) + r * a.ldl;
+                const float over = (float)((double)f / sum);
 #pragma unroll 1
-                for (int i = threadIdx.x; i < a.C; i += 1024) d[i] = (TD)(f == 0.f ? 0.f : (i == (int)lab ? f : 0.f) - __expf((float)z[i] - lse) * f);
+                for (int i = threadIdx.x; i < a.C; i += 1024)
+                    d[i] = (TD)(f == 0.f ? 0.f : (i == (int)lab ? f : 0.f) - __expf((float)z[i] - top) * over);
             }
         // (a ticket among few workgroups; the part is where every CU sees it before the ticket counts it)
         if (threadIdx.x == 0) {
@@ -653,7 +694,7 @@ inline unsigned grid_of(int64_t n, int64_t cap) { return (unsigned)(n < 1 ? 1 : 
 // what every entry asks of the rows; `grad` may be null
 int check_rows(const void *logits, int dtype, int64_t ldl, const int64_t *labels, int64_t M, int64_t C, const void *grad, int grad_dtype) {
     if (!is_dt(dtype) || (grad && !is_dt(grad_dtype)) || M < 0 || C <= 0 || ldl < C) return EMADAPT_ERR_INVALID;
-    if (ldl > (int64_t)1 << 30 || M > (int64_t)1 << 40) return EMADAPT_ERR_UNSUPPORTED;
+    if (ldl > (int64_t)1 << 30 || M > ((int64_t)1 << 48) / ldl) return EMADAPT_ERR_UNSUPPORTED;
     if (M == 0) return EMADAPT_OK;
     if (!logits || !labels || !aligned(logits, dt_size(dtype)) || !aligned(labels, 8) || (grad && !aligned(grad, dt_size(grad_dtype)))) return EMADAPT_ERR_INVALID;
     // (the rows are read again after other rows' gradients are written)
@@ -689,7 +730,7 @@ bool launch_short(const Rows &a, const Policy &p, const Outputs &out, int cap, i
 template <int MODE, typename T, typename TD>
 bool launch_block(const Rows &a, const Policy &p, const Outputs &out, int cap, int *blocks, hipStream_t stream) {
     const int64_t nvec = a.C / Vec<T>::N;
-    if (nvec > 16384) return false;
+    if (nvec < 1 || nvec > 16384) return false;   // (a thread without a vector of its own loads the row's last whole one: there has to be one)
     *blocks = (int)grid_of(a.M, cap);
     const dim3 grid(*blocks);
 #define EMADAPT_BLOCK(W, NV) hipLaunchKernelGGL((block_kernel<T, TD, W, NV, MODE>), grid, dim3(64 * W), 0, stream, a, p, out)
@@ -856,7 +897,7 @@ int emadapt_policy_loss(const void *logits, int dtype, int64_t ldl, const int64_
                         const float *weights, int64_t M, int64_t C, double clip_low, double clip_high, float kl_coef, float grad_scale, float *sums, float *logp,
                         void *dlogits, int dlogits_dtype, void *workspace, size_t workspace_bytes, void *stream_) {
     if (int rc = check_rows(logits, dtype, ldl, actions, M, C, dlogits, dlogits_dtype)) return rc;
-    if (!sums || !(clip_low >= 0.0 && clip_low <= 1.0) || !(clip_high >= 0.0)) return EMADAPT_ERR_INVALID;
+    if (!sums || !(clip_low >= 0.0 && clip_low <= 1.0) || !(clip_high >= 0.0) || !isfinite(kl_coef) || !isfinite(grad_scale)) return EMADAPT_ERR_INVALID;
     if (M && (!old_logp || !advantages || !logp)) return EMADAPT_ERR_INVALID;
     if (!workspace || !aligned(workspace, 8) || workspace_bytes < emadapt_policy_loss_workspace_bytes(M, C)) return EMADAPT_ERR_WORKSPACE;
     hipStream_t stream = as_stream(stream_);
@@ -876,7 +917,7 @@ int emadapt_preference_loss(const void *logits, int dtype, int64_t ldl, const in
                             int64_t M, int64_t C, float beta, float label_smoothing, float grad_scale, float *loss, float *seq_logp, void *dlogits,
                             int dlogits_dtype, void *workspace, size_t workspace_bytes, void *stream_) {
     if (int rc = check_rows(logits, dtype, ldl, labels, M, C, dlogits, dlogits_dtype)) return rc;
-    if (pairs < 0 || !(label_smoothing >= 0.f && label_smoothing <= 1.f)) return EMADAPT_ERR_INVALID;
+    if (pairs < 0 || !(label_smoothing >= 0.f && label_smoothing <= 1.f) || !isfinite(beta) || !isfinite(grad_scale)) return EMADAPT_ERR_INVALID;
     if (pairs > 0x7FFFFFFF) return EMADAPT_ERR_UNSUPPORTED;
     if (pairs && (!seq_start || !aligned(seq_start, 8) || !ref_logp || !loss || !seq_logp)) return EMADAPT_ERR_INVALID;
     if (M && (!workspace || !aligned(workspace, 4) || workspace_bytes < emadapt_preference_loss_workspace_bytes(M, C))) return EMADAPT_ERR_WORKSPACE;

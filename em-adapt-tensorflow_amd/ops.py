@@ -1040,10 +1040,12 @@ class AdamW:
         self.steps = self._control[:8].view(torch.int64)
         self.grad_norm = self._control[8:12].view(torch.float32)
         self._control_bytes = self._control.numel()
+        self._tables = {}   # by the gradients' type: the table on the device, the gradients
         self.set_grads(grads)
 
     def set_grads(self, grads):
-        """The gradients that step() reads from now on (a copy of their addresses goes to the device; not under graph capture)."""
+        """The gradients that step() reads from now on, also in a replay of a step that was captured with gradients of this type.  (Their addresses are
+        copied to the device, behind all work that is queued there: not under graph capture.)"""
         grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError("%d gradients for %d tensors" % (len(grads), len(self.params)))
@@ -1069,14 +1071,21 @@ class AdamW:
             raise _lib.EmadaptError(int(chunks), "emadapt_adamw_chunks")
         host = torch.zeros(lib.emadapt_adamw_table_bytes(chunks), dtype=torch.uint8)
         _lib.call("emadapt_adamw_table", len(grads), arr, dt, ADAMW_STATES[self.state], ctypes.c_void_p(host.data_ptr()), host.numel())
-        self.grads, self._gdt, self._chunks = grads, dt, chunks
+        _refuse_shared(self.params, "params", grads, "grads")
+        torch.cuda.synchronize(self.device)   # (a step on any stream may still be reading the table)
+        if dt in self._tables:
+            self._tables[dt][0].copy_(host)
+        else:
+            self._tables[dt] = [host.to(self.device), None]
+        self._tables[dt][1] = grads   # (a table's tensors live as long as it does)
+        self.grads, self._gdt, self._chunks, self._table = grads, dt, chunks, self._tables[dt][0]
         self._grads_apart = None
-        self._table = host.to(self.device)
 
     def step(self, lr, grad_scale=1.0, max_norm=0.0, zero_grads=False):
-        """One step: gradients times grad_scale, held to the global norm max_norm (0: not), weights and moments updated in place.  zero_grads: the
+        """One step on the current stream (steps of one object belong on one stream, or in order): gradients times grad_scale, held to the global norm max_norm (0: not), weights and moments updated in place.  zero_grads: the
         gradients are zeroed behind it.  A gradient (or norm) that is not finite leaves its elements (or the whole step) out and raises
-        STATUS_NAN_GRADIENT of the device status word; while the word is raised the step does nothing (status_poll)."""
+        STATUS_NAN_GRADIENT of the device status word; while the word is raised the step does nothing (status_poll).  A captured step replays with the
+        lr, grad_scale and max_norm of its capture, and counts on."""
         if zero_grads and not self._grads_apart:
             _refuse_overlap(self.grads, "grads")
             self._grads_apart = True
@@ -1118,6 +1127,17 @@ def _refuse_overlap(tensors, name):
     for (a, n, i), (b, _, j) in zip(spans, spans[1:]):
         if a + n > b:
             raise ValueError("%s[%d] and %s[%d] share memory" % (name, i, name, j))
+
+
+def _refuse_shared(a, a_name, b, b_name):
+    """No tensor of one list may share memory with one of the other (within a list they may)."""
+    spans = sorted((t.data_ptr(), side, t.numel() * t.element_size(), k) for side, ts in enumerate((a, b)) for k, t in enumerate(ts) if t.numel())
+    end = [(0, 0), (0, 0)]   # furthest end of either list so far, and whose it is
+    for at, side, n, k in spans:
+        if end[1 - side][0] > at:
+            i, j = (end[0][1], k) if side else (k, end[1][1])
+            raise ValueError("%s[%d] and %s[%d] share memory" % (a_name, i, b_name, j))
+        end[side] = max(end[side], (at + n, k))
 
 
 def status_word():

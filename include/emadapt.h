@@ -550,14 +550,16 @@ int emadapt_sgd_accumulate_pack(const float *g, const float *w, int64_t n, int64
  *            whatever the row's logits hold (infinities and NaN included)
  *   dlogits  f32 or bf16 [M][ldl], written as a whole: the padding columns and the rows that take no part become 0.  It must not
  *            overlap the logits (EMADAPT_ERR_INVALID)
- * A logit of -inf is a class of probability 0.  Arithmetic is f32, sums over rows f64 in a fixed order: results are bit-identical from
- * run to run.  The reference has no counterpart (its one loss is the cross-entropy of deeplab.py:182).
+ * A logit of -inf is a class of probability 0 (a row of nothing else that has a label has no distribution: NaN); a row masked as a whole
+ * with the type's lowest value is an even one.  Arithmetic is f32, sums over rows f64 in a fixed order: results are bit-identical from
+ * run to run.  Scalars that are not finite (kl_coef, grad_scale, beta) are refused.  The reference has no counterpart (its one loss is the cross-entropy of deeplab.py:182).
  * ---------------------------------------------------------------------------------------- */
 
 /* lse[r] = log sum_{c < C} exp(logits[r][c]);  logp[r] = logits[r][labels[r]] - lse[r].  Either output may be NULL. */
 int emadapt_label_logp(const void *logits, int dtype, int64_t ldl, const int64_t *labels, int64_t M, int64_t C, float *logp, float *lse,
                        void *stream);
-/* dlogits[r][c] = ([c == labels[r]] - exp(logits[r][c] - lse[r])) * dlogp[r]; a row with dlogp 0 is 0. */
+/* dlogits[r][c] = ([c == labels[r]] - exp(logits[r][c] - lse[r])) * dlogp[r]; a row with dlogp 0 is 0.  Where |lse| >= 4096 (its f32 value then
+ * lacks the sum's last bits) and lse is the row's own to rounding, the sum is taken anew. */
 int emadapt_label_logp_bwd(const void *logits, int dtype, int64_t ldl, const int64_t *labels, const float *lse, const float *dlogp,
                            int64_t M, int64_t C, void *dlogits, int dlogits_dtype, void *stream);
 
@@ -602,7 +604,8 @@ int emadapt_preference_loss(const void *logits, int dtype, int64_t ldl, const in
  * replayed; two steps on one control block belong on one stream.
  * A raised status word makes the step a no-op (not in collective mode: the gradient carries the failure).  A norm that is not finite
  * makes the step a no-op; an element whose moments would leave the finite numbers is left alone; both raise EMADAPT_STATUS_NAN_GRADIENT.
- * zero_grads: the gradients are zeroed behind the step (the clean op of deeplab.py:204).  beta1, beta2 in [0, 1), eps >= 1e-16. */
+ * zero_grads: the gradients are zeroed behind the step (the clean op of deeplab.py:204).  beta1, beta2 in [0, 1), eps >= 1e-16; lr, grad_scale,
+ * weight_decay and lr_scale finite. */
 #define EMADAPT_ADAMW_F32 0
 #define EMADAPT_ADAMW_U8 1
 typedef struct emadapt_adamw_tensor {
@@ -622,7 +625,7 @@ int emadapt_adamw_step(const void *table, int64_t chunks, int grad_dtype, int st
                        double beta1, double beta2, double eps, float grad_scale, double max_norm, unsigned seed, int zero_grads,
                        void *stream);
 /* 8-bit states <-> values (checkpoints): n a multiple of 64; u = sqrt(v).  unpack writes f32 or bf16 (exact in both); pack rounds to
- * nearest and gives back what unpack gave. */
+ * nearest, holds values to the formats' largest, takes NaN as 0, and gives back what unpack gave. */
 int emadapt_adamw_unpack(const void *m_codes, const void *u_codes, const void *powers, int64_t n, void *m, void *u, int dtype, void *stream);
 int emadapt_adamw_pack(const float *m, const float *u, int64_t n, void *m_codes, void *u_codes, void *powers, void *stream);
 

@@ -351,3 +351,51 @@ def test_refusals(env):
             call()
     with pytest.raises(ops._lib.EmadaptError):
         ops.AdamW([w], [g]).step(1e-3, max_norm=-1.0)
+
+
+def test_new_gradients_reach_a_captured_step(env):
+    """set_grads() after a capture: replays read the new gradients (of the type they were captured with), never an address that is gone."""
+    ops, torch = env
+    for state in ("f32", "u8"):
+        ws, gs = _tensors(torch, [700, 4097, 64], "float32", 13)
+        ours = ops.AdamW([w.clone() for w in ws], [g.clone() for g in gs], state=state, seed=3)
+        eager = ops.AdamW([w.clone() for w in ws], gs, state=state, seed=3)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ours.step(1e-3, max_norm=0.1)
+        narrow = [(g * 0.5).bfloat16() for g in gs]
+        for turn in range(3):
+            for o in (ours, eager):
+                o.set_grads(narrow)
+                o.step(1e-3, max_norm=0.1)
+            fresh = [g * (turn - 1.5) for g in gs]
+            ours.set_grads([g.clone() for g in fresh])
+            graph.replay()
+            torch.cuda.synchronize()
+            eager.set_grads(fresh)
+            eager.step(1e-3, max_norm=0.1)
+            assert int(ours.steps) == int(eager.steps) == 2 * turn + 2
+            assert all(torch.equal(a, b) for a, b in zip(ours.params, eager.params)), (state, turn)
+
+
+def test_gradients_in_the_weights_are_refused(env):
+    ops, torch = env
+    w, g = torch.zeros(100, device="cuda"), torch.zeros(100, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        ops.AdamW([w], [w])
+    opt = ops.AdamW([w[:50], w[50:]], [g[:50], g[50:]])
+    with pytest.raises(ValueError, match="share memory"):
+        opt.set_grads([g[:50], w[10:60]])
+    opt.step(1e-3)
+
+
+def test_pack_takes_nan_as_zero(env):
+    ops, torch = env
+    opt = ops.AdamW([torch.zeros(128, device="cuda")], [torch.zeros(128, device="cuda")], state="u8")
+    m, u = torch.ones(opt.total, device="cuda"), torch.ones(opt.total, device="cuda")
+    m[3] = u[3] = m[70] = float("nan")
+    m[5], u[5] = float("inf"), float("inf")
+    opt.pack(m, u)
+    m2, u2 = opt.unpack()
+    assert float(m2[3]) == 0 and float(u2[3]) == 0 and float(m2[70]) == 0 and float(u2[70]) == 1
+    assert bool(torch.isfinite(m2).all()) and bool(torch.isfinite(u2).all()) and bool((m2[64:70] == 1).all())

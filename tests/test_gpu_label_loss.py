@@ -429,3 +429,97 @@ def test_on_another_stream_and_in_a_replayed_graph(env):
         torch.cuda.synchronize()
         for (_, call), (_, out) in zip(cases, graphs):
             assert all(torch.equal(x, y) for x, y in zip(call(), out)), turn
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("M,C,ldl", [(5, 3, 600), (9, 1, 5000), (40, 7, 300), (2, 5, 140001), (300, 8, 1001)])
+def test_few_classes_in_long_rows(env, M, C, ldl, dtype):
+    """Fewer classes than one 16-byte load holds, in rows far longer: no load may start in front of the row or behind it."""
+    ops, torch = env
+    _say("few classes", M, C, ldl, dtype)
+    z = _logits(torch, M, ldl, dtype, M + ldl, offset=1)
+    z[:, C:] = float("nan")
+    lab = _labels(torch, M, C, M, outside=False)
+    logp, lse = ops.label_logp(z, lab, C)
+    x, want_lse, want, used, tol = _reference(torch, z, lab, C)
+    at = x.gather(1, lab[:, None])[:, 0].abs()
+    assert bool(((logp.double() - want).abs() <= tol + H * (at + want.abs())).all())
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    adv = torch.randn(M, generator=gen, device="cuda")
+    old = (want + 0.1).float()
+    sums, lp, d = ops.policy_loss(z, lab, old, adv, C, grad_scale=1.0)
+    x, _, want_lp, used, lp_tol, tol, wsums, wsums_tol, coef, coef_tol = _policy_reference(torch, z, lab, old, adv, C, None, None, 0.2, 0.2, 0.0, 1.0)
+    assert bool(((sums.double() - wsums).abs() <= wsums_tol).all())
+    _check_grad(torch, d, x, want_lse, used, lab, coef, coef_tol, tol, C)
+    at, ref = torch.tensor([0, M // 2, M], device="cuda"), torch.zeros(2, device="cuda")
+    loss, seq, d = ops.preference_loss(z, lab, at, ref, C, grad_scale=1.0)
+    x, _, used, tol, wseq, seq_tol, wloss, loss_tol, coef, coef_tol = _preference_reference(torch, z, lab, at, ref, C, 0.1, 0.0, 1.0)
+    assert bool(((loss.double() - wloss).abs() <= loss_tol).all())
+    _check_grad(torch, d, x, want_lse, used, lab, coef, coef_tol, tol, C)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("M,C,ldl", [(300, 21, 24), (6, 700, 700), (3, 5001, 5001), (2, 130001, 130001)])
+def test_gradient_far_from_zero(env, M, C, ldl, dtype):
+    """Rows whose log-sum-exp in f32 lacks the sum's bits: the gradient is the row's own all the same.  Maximum and sum are then taken in the gradient's
+    launch (differences to the maximum rounded once), so |lse| and |max| leave the tolerance."""
+    ops, torch = env
+    _say("far", M, C, dtype)
+    z = _logits(torch, M, ldl, dtype, C)
+    lo = torch.finfo(z.dtype).min
+    for r in range(M):
+        z[r] = (z[r].float() + (5000.0, -5000.0, 1e6)[r % 3]).to(z.dtype) if r % 4 else lo
+    lab = _labels(torch, M, C, C, outside=False)
+    _, lse = ops.label_logp(z, lab, C)
+    x = z[:, :C].double()
+    x = x - x.amax(1, keepdim=True)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    coef = torch.randn(M, generator=gen, device="cuda")
+    d = ops.label_logp_bwd(z, lab, lse, coef, C)
+    n = C / (64 if C > 512 else 4) + 1
+    tol = H * (n + 32 + 3 * (x.amax(1) - x.amin(1)))
+    _check_grad(torch, d, x, torch.logsumexp(x, 1), torch.ones_like(lab, dtype=torch.bool), lab, coef.double(), torch.zeros_like(tol), tol, C)
+    # a log-sum-exp that is not the row's own (the classes are a part of all) is taken as it is: off by half a step of itself
+    other = lse + 1.0 + lse.abs() * 2.0 ** -20
+    d = ops.label_logp_bwd(z, lab, other, coef, C)
+    full = z[:, :C].double()
+    sane = lse.abs() < 1e30
+    _check_grad(torch, d[sane], full[sane], other[sane].double(), sane[sane], lab[sane], coef[sane].double(), torch.zeros_like(tol[sane]), (H * 4 * other.abs().double())[sane], C)
+
+
+@pytest.mark.parametrize("M,C,ldl", [(300, 21, 24), (20, 700, 700), (200, 5001, 5001), (3, 40000, 40000), (2, 300001, 300001)])
+def test_policy_of_an_action_at_the_lowest_value(env, M, C, ldl):
+    """clip_low 0 puts the border at ratio 1: all rows with old_logp = logp lie on it, also those whose action is masked with the type's lowest value
+    (log-probability -3.4e38, ratio 1 all the same) or far below the others."""
+    ops, torch = env
+    z = _logits(torch, M, ldl, "float32", 6)
+    lab = _labels(torch, M, C, 6, outside=False)
+    rows = torch.arange(M, device="cuda")
+    z[rows[::2], lab[::2]] = torch.finfo(torch.float32).min
+    z[rows[1::2], lab[1::2]] = -1000.0
+    logp = _reference(torch, z, lab, C)[2].float()
+    adv = -torch.ones(M, device="cuda")
+    for want_grad in (False, True):
+        sums, lp, d = ops.policy_loss(z, lab, logp, adv, C, clip_low=0.0, grad_scale=1.0, want_grad=want_grad)
+        # a ratio is off by exp(half a step of logp near 1000) at most; where f32 logp is above the exact one the ratio is below 1 and held there
+        assert abs(float(sums[0]) - M) <= M * 2 * H * 1100
+        assert bool(((lp - logp).abs() <= 2 * H * logp.abs()).all())
+    x = z[:, :C].double()
+    p = torch.softmax(x, 1)
+    hot = torch.zeros_like(p)
+    hot[rows, lab] = 1.0
+    free = d[rows, lab] != 0
+    assert bool(free[::2].all())
+    assert bool(((d[:, :C].double() - (hot - p) * free[:, None]).abs() <= 1e-3 * (hot - p).abs() + 1e-38).all())
+
+
+def test_kl_of_weight_zero_does_not_count(env):
+    ops, torch = env
+    for M, C in ((50, 21), (9, 5000), (2, 200001)):
+        z = _logits(torch, M, C, "float32", 1)
+        lab = _labels(torch, M, C, 1, outside=False)
+        logp = ops.label_logp(z, lab, C)[0]
+        adv = torch.ones(M, device="cuda")
+        a = ops.policy_loss(z, lab, logp - 0.05, adv, C, kl_coef=0.0)
+        b = ops.policy_loss(z, lab, logp - 0.05, adv, C, ref_logp=logp + 120.0, kl_coef=0.0)   # exp(120) is beyond f32
+        assert torch.equal(a[0][:2], b[0][:2]) and torch.equal(a[2], b[2]) and bool(torch.isfinite(b[2]).all())

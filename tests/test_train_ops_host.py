@@ -152,3 +152,31 @@ def test_wrappers_refuse_cpu_tensors():
         ops.AdamW([torch.zeros(4)], [torch.zeros(4)])
     with pytest.raises(ValueError):
         ops.AdamW([], [])
+
+
+def test_scalars_that_are_not_finite_are_refused(lib):
+    big, size = 1 << 30, lib.emadapt_adamw_control_bytes()
+    for bad in (float("nan"), float("inf")):
+        for kl, scale in ((bad, 1.0), (0.1, bad)):
+            assert lib.emadapt_policy_loss(1 << 20, 0, 24, 8192, big, big, big, None, 4, 21, 0.2, 0.2, kl, scale, big, big, None, 0, big, 1 << 20, None) == INVALID
+        for beta, scale in ((bad, 1.0), (0.1, bad)):
+            assert lib.emadapt_preference_loss(1 << 20, 0, 24, 8192, big, 2, big, 4, 21, beta, 0.0, scale, big, big, None, 0, big, 1 << 20, None) == INVALID
+        for lr, scale in ((bad, 1.0), (1e-3, bad)):
+            assert lib.emadapt_adamw_step(4096, 1, 0, 0, 8192, size, lr, 0.9, 0.999, 1e-8, scale, 0.0, 0, 0, None) == INVALID
+        assert _table(lib, [_tensor(5, wd=bad)])[0] == INVALID and _table(lib, [_tensor(5, ls=bad)])[0] == INVALID
+
+
+def test_rows_beyond_any_memory_are_refused(lib):
+    assert _logp(lib, ldl=1 << 30, C=21, M=1 << 39) == UNSUPPORTED
+
+
+def test_tensors_of_two_lists_may_not_share_memory():
+    import torch
+    from em_adapt_tensorflow_amd import ops
+    room = torch.zeros(100)
+    a, b = [room[:10], room[40:60]], [room[10:40], room[10:20], room[60:]]
+    ops._refuse_shared(a, "params", b, "grads")
+    for more in (room[5:6], room[30:41], room[59:61], room):
+        with pytest.raises(ValueError, match="share memory"):
+            ops._refuse_shared(a, "params", b + [more], "grads")
+    ops._refuse_shared(a, "params", b + [room[50:50]], "grads")
