@@ -123,11 +123,12 @@ struct Rows {
 };
 
 // An f32 log-sum-exp of this size and more keeps too little of the sum (2^-12 of a probability is rounding here, and of a row masked as a whole with
-// the type's lowest value the log C is gone): one wave takes the rows' maxima and sums anew, one row after the other, for its lanes.  A lane whose
-// lse is not the one of its row (a part of the classes, say) keeps it.
+// the type's lowest value the log C is gone): one wave takes the rows' maxima and sums anew, one row after the other, for its lanes.  False: no such
+// row, or its lse is not its own (of a part of the classes, say).
 constexpr float kFar = 4096.f;
 template <typename T>
-__device__ void sums_anew(const Rows &a, long long row, bool far, float f, float &base, float &fs) {
+__device__ bool sum_anew(const Rows &a, long long row, bool far, float lse, MaxSum &own) {
+    bool anew = false;
     for (unsigned long long left = __ballot(far); left;) {
         const long long r = __shfl(row, __ffsll((long long)left) - 1);
         const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
@@ -139,59 +140,76 @@ __device__ void sums_anew(const Rows &a, long long row, bool far, float f, float
         for (int i = threadIdx.x & 63; i < a.C; i += 64) s += __expf((float)z[i] - m);
         s = group_sum<64>(s);
         const bool mine = far && row == r;
-        if (mine && fabsf(m + logf(s) - base) <= 0x1p-22f * fabsf(base)) {
-            base = m;
-            fs = f / s;
+        if (mine && fabsf(m + logf(s) - lse) <= 0x1p-22f * fabsf(lse)) {
+            own = {m, s};
+            anew = true;
         }
         left &= ~__ballot(mine);
     }
+    return anew;
 }
 
-// dz = [c = label] coef - exp(z - base) coef / sum (base, sum: the row's maximum and sum; without sum the log-sum-exp): every thread kUnroll vectors
-// of the flattened [M][vectors per row], all in flight.  A workgroup's vectors lie behind one another; their rows come from one 64-bit division for
-// the workgroup and a 32-bit one for each vector.
-template <typename T, typename TD, int kUnroll>
+// dz = [c = label] coef - exp(z - base) coef / sum (base, sum: the row's maximum and sum; without SUM base is the log-sum-exp): every thread kUnroll
+// vectors of the flattened [M][vectors per row], all in flight.  A workgroup's vectors lie behind one another; their rows come from one 64-bit
+// division for the workgroup and a 32-bit one for each vector.  Rows far from zero are written again at the end (looked at in front of the store
+// they cost the others 4 to 9 % of the time).
+template <typename T, typename TD, int kUnroll, bool SUM>
 __global__ void __launch_bounds__(256) row_grad_kernel(Rows a, const float *__restrict__ base, const float *__restrict__ sum, const float *__restrict__ coef, TD *__restrict__ dlogits,
                                                       unsigned nvec, long long total) {
     constexpr int N = Vec<T>::N;
     const long long b = (long long)(gridDim.x - 1 - blockIdx.x) * (256 * kUnroll);   // (the rows that were read last come first: some are still in the cache)
     const long long r0 = b / nvec;
     const unsigned i0 = (unsigned)(b - r0 * nvec);
+    struct Place {
+        long long row;   // -1: past the end
+        int at;
+    };
+    auto place = [&](int q) {
+        const unsigned o = i0 + q * 256 + threadIdx.x, dr = o / nvec;
+        return Place{b + q * 256 + threadIdx.x < total ? r0 + dr : -1, (int)(o - dr * nvec) * N};
+    };
     Raw raw[kUnroll];
-    long long row[kUnroll];
-    int at[kUnroll], hit[kUnroll];
+    Place to[kUnroll];
+    int hit[kUnroll];
     float l[kUnroll], f[kUnroll], fs[kUnroll];
 #pragma unroll
     for (int q = 0; q < kUnroll; q++) {
-        const unsigned o = i0 + q * 256 + threadIdx.x, dr = o / nvec;
-        row[q] = b + q * 256 + threadIdx.x < total ? r0 + dr : -1;
-        if (row[q] < 0) continue;
-        at[q] = (int)(o - dr * nvec) * N;
-        raw[q] = load_row<false>(static_cast<const T *>(a.logits) + row[q] * a.ldl, at[q], a.C, (int)a.ldl);
-        const long long lab = a.labels[row[q]];
+        to[q] = place(q);
+        const long long row = to[q].row;
+        if (row < 0) continue;
+        raw[q] = load_row<false>(static_cast<const T *>(a.logits) + row * a.ldl, to[q].at, a.C, (int)a.ldl);
+        const long long lab = a.labels[row];
         const bool used = lab >= 0 && lab < a.C;
         hit[q] = used ? (int)lab : -(1 << 30);
-        l[q] = base[row[q]];
-        f[q] = used ? coef[row[q]] : 0.f;
-        fs[q] = sum ? f[q] * __builtin_amdgcn_rcpf(sum[row[q]]) : f[q];
+        l[q] = base[row];
+        f[q] = used ? coef[row] : 0.f;
+        fs[q] = SUM ? f[q] * __builtin_amdgcn_rcpf(sum[row]) : f[q];
     }
-    if (!sum) {
-#pragma unroll
-        for (int q = 0; q < kUnroll; q++) {
-            const bool far = row[q] >= 0 && f[q] != 0.f && fabsf(l[q]) >= kFar && fabsf(l[q]) < INFINITY;
-            if (__any(far)) sums_anew<T>(a, row[q], far, f[q], l[q], fs[q]);
-        }
-    }
+    unsigned far = 0u;
 #pragma unroll
     for (int q = 0; q < kUnroll; q++) {
-        if (row[q] < 0) continue;
+        const long long row = to[q].row;
+        if (row < 0) continue;
+        if (!SUM) far |= f[q] != 0.f && fabsf(l[q]) >= kFar && fabsf(l[q]) < INFINITY ? 1u << q : 0u;
         float v[N];
-        grad_vec<T>(raw[q], l[q], fs[q], f[q], hit[q] - at[q], v);
+        grad_vec<T>(raw[q], l[q], fs[q], f[q], hit[q] - to[q].at, v);
         if (f[q] == 0.f) {   // (a row that takes no part: 0, also where 0 * NaN is not)
 #pragma unroll
             for (int k = 0; k < N; k++) v[k] = 0.f;
         }
-        store_row<TD>(dlogits + row[q] * a.ldl, at[q], (int)a.ldl, v, a.once);
+        store_row<TD>(dlogits + row * a.ldl, to[q].at, (int)a.ldl, v, a.once);
+    }
+    if (SUM || !__any(far != 0u)) return;
+#pragma unroll 1
+    for (int q = 0; q < kUnroll; q++) {
+        const bool mine = far >> q & 1u;
+        const Place t = place(q);
+        MaxSum own = {0.f, 1.f};
+        if (!sum_anew<T>(a, t.row, mine, mine ? base[t.row] : 0.f, own)) continue;
+        const float c = coef[t.row];
+        float v[N];
+        grad_vec<T>(load_row<false>(static_cast<const T *>(a.logits) + t.row * a.ldl, t.at, a.C, (int)a.ldl), own.m, c / own.s, c, (int)a.labels[t.row] - t.at, v);
+        store_row<TD>(dlogits + t.row * a.ldl, t.at, (int)a.ldl, v, false);
     }
 }
 
@@ -260,10 +278,10 @@ enum { kLogp = 0, kPolicy = 1, kPolicyGrad = 2 };
 constexpr int kSplits = 32;   // parts of a row where rows are few
 struct Outputs {
     float *logp, *lse;          // kLogp: any of these may be null
-    float *base, *sum, *zero;   // kLogp: the rows' maximum and sum of exponentials; a value per row set to 0
+    float *base, *sum, *zero;   // kLogp: the rows' maximum and sum of exponentials; a value per row set to 0 (kPolicyGrad: base of the near rows)
     void *dlogits;
     double *partial;            // a workgroup's sums, [gridDim.x][4]
-    unsigned char *near;        // rows to be looked at in 64 bits (policy_finish_kernel)
+    unsigned char *near;        // rows to be looked at in 64 bits from their maximum in base (policy_finish_kernel)
     unsigned *ticket;           // its ticket, to be zeroed
     MaxSum *parts;              // [M][gridDim.y] of rows in several parts
 };
@@ -451,7 +469,11 @@ __global__ void __launch_bounds__(64 * W, 4) block_kernel(Rows a, Policy p, Outp
                 terms.loss += one.loss; terms.surrogate += one.surrogate; terms.kl += one.kl; terms.clipped += one.clipped;
             }
         }
-        if (threadIdx.x == 0) { out.logp[r] = lp; out.near[r] = near; }
+        if (threadIdx.x == 0) {
+            out.logp[r] = lp;
+            out.near[r] = near;
+            if (near) out.base[r] = row.m;
+        }
         TD *d = static_cast<TD *>(out.dlogits) + r * a.ldl;
         const int hit = used ? (int)lab : -(1 << 30);
         const float fs = f * __builtin_amdgcn_rcpf(row.s);
@@ -595,7 +617,6 @@ template <typename T, typename TD>
 __global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, Outputs out, int nparts, double *__restrict__ fixed, float *__restrict__ sums) {
     __shared__ double sh[16][4];
     __shared__ double one[16];
-    __shared__ MaxSum pair[16];
     __shared__ unsigned long long mask[16];
     __shared__ bool last;
     PolicyTerms t = {0, 0, 0, 0};
@@ -608,10 +629,7 @@ __global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, O
             for (unsigned long long left = mask[q]; left; left &= left - 1) {
                 const long long r = r0 + q * 64 + (__ffsll((long long)left) - 1), lab = a.labels[r];
                 const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
-                float top = -INFINITY;
-#pragma unroll 1
-                for (int i = threadIdx.x; i < a.C; i += 1024) top = fmaxf(top, (float)z[i]);
-                top = block_join<16>(MaxSum{group_max<64>(top), 0.f}, pair).m;
+                const float top = out.base[r];
                 const double sum = block_sum_f64(exact_part(z, a.C, top, threadIdx.x, 1024), one), lp64 = exact_logp((float)z[lab], top, sum);
                 float lp;
                 const float f = policy_of_exact(p, policy_inputs(p, r), lp64, threadIdx.x == 0, lp, t);
@@ -772,13 +790,20 @@ int launch_grad_t(const Rows &a, const float *base, const float *sum, const floa
     const bool four = total >= 4 * 256 * 1024;
     const int64_t blocks = ceil_div(total, four ? 1024 : 256);
     if (blocks > 0x7FFFFFFF) return EMADAPT_ERR_UNSUPPORTED;
-#define EMADAPT_GRAD(TD, U) \
-    hipLaunchKernelGGL((row_grad_kernel<T, TD, U>), dim3((unsigned)blocks), dim3(256), 0, stream, a, base, sum, coef, static_cast<TD *>(d), (unsigned)nvec, (long long)total)
-    if (ddt == EMADAPT_DT_BF16) {
-        if (four) EMADAPT_GRAD(__bf16, 4); else EMADAPT_GRAD(__bf16, 1);
-    } else {
-        if (four) EMADAPT_GRAD(float, 4); else EMADAPT_GRAD(float, 1);
+#define EMADAPT_GRAD(TD, U, SUM) \
+    hipLaunchKernelGGL((row_grad_kernel<T, TD, U, SUM>), dim3((unsigned)blocks), dim3(256), 0, stream, a, base, sum, coef, static_cast<TD *>(d), (unsigned)nvec, (long long)total)
+#define EMADAPT_GRAD_OF(SUM)                                             \
+    if (ddt == EMADAPT_DT_BF16) {                                        \
+        if (four) EMADAPT_GRAD(__bf16, 4, SUM); else EMADAPT_GRAD(__bf16, 1, SUM); \
+    } else {                                                             \
+        if (four) EMADAPT_GRAD(float, 4, SUM); else EMADAPT_GRAD(float, 1, SUM);   \
     }
+    if (sum) {
+        EMADAPT_GRAD_OF(true)
+    } else {
+        EMADAPT_GRAD_OF(false)
+    }
+#undef EMADAPT_GRAD_OF
 #undef EMADAPT_GRAD
     return launch_status();
 }
@@ -834,6 +859,7 @@ int policy_t(Rows a, Policy p, float *sums, float *logp, void *dlogits, int ddt,
             done = launch_short<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
             if (!done && !few) {
                 out.near = w.near;
+                out.base = w.base;
                 done = launch_block<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
                 if (done) finish = (unsigned)ceil_div(a.M, 1024);
                 else out.near = nullptr;

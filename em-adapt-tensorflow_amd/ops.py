@@ -910,7 +910,8 @@ def label_logp(logits, labels, num_classes):
     """(logp f32 [...], lse f32 [...]): log-probability of the given labels and the rows' log-sum-exp.  logits f32 / bf16 [..., ldl], labels
     int64 [...]; a label outside [0, num_classes) has logp 0."""
     dt, ldl, M, C = _rows(logits, labels, num_classes)
-    logp, lse = _f32(labels.shape, logits), _f32(labels.shape, logits)
+    logp = _f32(labels.shape, logits)
+    lse = torch.empty_like(logp)
     _launch(logits, "emadapt_label_logp", logits.data_ptr(), dt, ldl, labels.data_ptr(), M, C, logp.data_ptr(), lse.data_ptr())
     return logp, lse
 
@@ -948,7 +949,7 @@ def policy_loss(logits, actions, old_logp, advantages, num_classes, ref_logp=Non
     ddt = DT_F32
     if want_grad:
         dlogits, ddt = _dlogits(logits, dt, dlogits)
-    sums, logp = _f32(4, logits), _f32(actions.shape, logits)
+    sums, logp = _f32(4, logits), torch.empty_like(old_logp) if old_logp.shape == actions.shape else _f32(actions.shape, logits)
     nbytes = _lib.load().emadapt_policy_loss_workspace_bytes(M, C)
     ws = _scratch(nbytes, logits)
     _launch(logits, "emadapt_policy_loss", logits.data_ptr(), dt, ldl, actions.data_ptr(), old, ref, adv, weight, M, C, clip_low, clip_high, kl_coef,
