@@ -113,6 +113,15 @@ template <int W> __device__ __forceinline__ MaxSum block_join(MaxSum wave, MaxSu
     r.s = group_sum<W>(t.s * __expf(t.m - finite_or_0(r.m)));
     return r;
 }
+// of a row's kSplits parts, by every kSplits lanes that call it together
+constexpr int kSplits = 32;   // parts of a row where rows are few
+__device__ __forceinline__ MaxSum join_parts(const MaxSum *parts) {
+    const MaxSum t = parts[threadIdx.x % kSplits];
+    MaxSum r;
+    r.m = group_max<kSplits>(t.m);
+    r.s = group_sum<kSplits>(t.s * __expf(t.m - finite_or_0(r.m)));
+    return r;
+}
 struct Rows {
     const void *logits;
     const long long *labels;
@@ -275,7 +284,6 @@ __device__ __forceinline__ double exact_logp(float z, float top, double sum) { r
 // rows that stay in registers: one pass over the logits
 // ------------------------------------------------------------------------------------------
 enum { kLogp = 0, kPolicy = 1, kPolicyGrad = 2 };
-constexpr int kSplits = 32;   // parts of a row where rows are few
 struct Outputs {
     float *logp, *lse;          // kLogp: any of these may be null
     float *base, *sum, *zero;   // kLogp: the rows' maximum and sum of exponentials; a value per row set to 0 (kPolicyGrad: base of the near rows)
@@ -529,7 +537,7 @@ __global__ void __launch_bounds__(64 * W) stream_stats_kernel(Rows a, Outputs ou
                 take(v, m, s);
             }
         }
-        for (; i0 < end; i0 += kThreads * N) {
+        for (; i0 < end; i0 += kThreads * N) {   // (one at a time: all of the rest in flight costs 16 waves the second workgroup on a CU, 31 -> 39 us for 3000 x 32768)
             float v[N];
             unpack<T>(load_row<ONCE>(z, i0, end, end), v);
             take(v, m, s);
@@ -548,40 +556,34 @@ __global__ void __launch_bounds__(64 * W) stream_stats_kernel(Rows a, Outputs ou
     }
 }
 
-// The rows' terms where the log-sum-exp comes from a launch of its own, as the rows' maximum and sum or in kSplits parts of each row.  One
-// workgroup also writes the sums.
-template <typename T>
-__global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const MaxSum *__restrict__ parts, float *__restrict__ base,
-                                                        float *__restrict__ sum, float *__restrict__ logp, float *__restrict__ coef,
-                                                        double *__restrict__ partial, float *__restrict__ sums) {
+// The rows' terms where the log-sum-exp comes from a launch of its own: as the rows' maximum and sum, or (PARTS) in kSplits parts of each row.
+// By workgroup `block` of `blocks`; a single one also writes the sums.
+template <typename T, bool PARTS>
+__device__ void policy_rows(const Rows &a, const Policy &p, const MaxSum *__restrict__ parts, const float *__restrict__ base, const float *__restrict__ sum,
+                            float *__restrict__ logp, float *__restrict__ coef, double *__restrict__ partial, float *__restrict__ sums, unsigned block, unsigned blocks) {
     __shared__ double sh[4];
     __shared__ unsigned long long mask[4];
-    __shared__ MaxSum whole[256];
+    __shared__ MaxSum whole[PARTS ? 256 : 1];
     PolicyTerms t = {0, 0, 0, 0};
-    for (long long r0 = (long long)blockIdx.x * 256; r0 < a.M; r0 += (long long)gridDim.x * 256) {
+    for (long long r0 = (long long)block * 256; r0 < a.M; r0 += (long long)blocks * 256) {
         const long long r = r0 + threadIdx.x;
         bool again = false;
-        if (parts) {   // a lane to a part, kSplits of them to a row
+        if (PARTS) {   // a lane to a part
             for (int q = threadIdx.x / kSplits; q < 256 && r0 + q < a.M; q += 256 / kSplits) {
-                const MaxSum part = parts[(r0 + q) * kSplits + threadIdx.x % kSplits];
-                const float m = group_max<kSplits>(part.m), s = group_sum<kSplits>(part.s * __expf(part.m - finite_or_0(m)));
-                if (threadIdx.x % kSplits == 0) {
-                    whole[q] = {m, s};
-                    base[r0 + q] = m;
-                    sum[r0 + q] = s;
-                }
+                const MaxSum row = join_parts(parts + (r0 + q) * kSplits);
+                if (threadIdx.x % kSplits == 0) whole[q] = row;
             }
             __syncthreads();
         }
         if (r < a.M) {
             const long long lab = a.labels[r];
             const float w = p.weight ? p.weight[r] : 1.f;
-            const MaxSum row = parts ? whole[threadIdx.x] : MaxSum{base[r], sum[r]};
+            const MaxSum row = PARTS ? whole[threadIdx.x] : MaxSum{base[r], sum[r]};
             float lp = 0.f, f = 0.f;
             if (lab >= 0 && lab < a.C && w != 0.f)
                 f = policy_of_row(p, policy_inputs(p, r), (float)(static_cast<const T *>(a.logits) + r * a.ldl)[lab], row, true, lp, again, t);
             logp[r] = lp;
-            coef[r] = f;
+            if (!PARTS) coef[r] = f;
         }
         // rows near a border, in the order of their index
         const unsigned long long b = __ballot(again);
@@ -589,14 +591,16 @@ __global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const
         __syncthreads();
         for (int q = 0; q < 4; q++)
             for (unsigned long long left = mask[q]; left; left &= left - 1) {
-                const long long rr = r0 + q * 64 + (__ffsll((long long)left) - 1);
+                const int k = q * 64 + (__ffsll((long long)left) - 1);
+                const long long rr = r0 + k;
                 const T *z = static_cast<const T *>(a.logits) + rr * a.ldl;
-                const float top = base[rr];
+                const float top = PARTS ? whole[k].m : base[rr];
                 const double lp64 = exact_logp((float)z[a.labels[rr]], top, block_sum_f64(exact_part(z, a.C, top, threadIdx.x, 256), sh));
                 if (threadIdx.x == 0) {
                     float lp;
-                    coef[rr] = policy_of_exact(p, policy_inputs(p, rr), lp64, true, lp, t);
+                    const float f = policy_of_exact(p, policy_inputs(p, rr), lp64, true, lp, t);
                     logp[rr] = lp;
+                    if (!PARTS) coef[rr] = f;
                 }
             }
         __syncthreads();
@@ -605,9 +609,55 @@ __global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const
     for (int k = 0; k < 4; k++) {
         const double v = block_sum_f64(s[k], sh);
         if (threadIdx.x == 0) {
-            if (gridDim.x == 1) sums[k] = (float)v;
-            else partial[(long long)blockIdx.x * 4 + k] = v;
+            if (blocks == 1) sums[k] = (float)v;
+            else partial[(long long)block * 4 + k] = v;
         }
+    }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const float *__restrict__ base, const float *__restrict__ sum, float *__restrict__ logp,
+                                                        float *__restrict__ coef, double *__restrict__ partial, float *__restrict__ sums) {
+    policy_rows<T, false>(a, p, nullptr, base, sum, logp, coef, partial, sums, blockIdx.x, gridDim.x);
+}
+// Few long rows, whose statistics came in parts: the first workgroup writes logp and the sums, the others the gradient of 256 kUnroll vectors of
+// one row each (per: workgroups to a row), whose term each of them takes from the parts by itself -- a launch less than with the terms in one of
+// their own (7 rows of 128001 bf16: 20.9 us and 17.5, 128 rows: 35 and 26).  In a row near a border each of them goes through the row.
+template <typename T, typename TD, int kUnroll>
+__global__ void __launch_bounds__(256) policy_few_kernel(Rows a, Policy p, const MaxSum *__restrict__ parts, float *__restrict__ logp, float *__restrict__ sums,
+                                                        TD *__restrict__ dlogits, unsigned per) {
+    constexpr int N = Vec<T>::N;
+    __shared__ double sh[4];
+    if (blockIdx.x == 0) {
+        policy_rows<T, true>(a, p, parts, nullptr, nullptr, logp, nullptr, nullptr, sums, 0, 1);
+        return;
+    }
+    const long long r = (blockIdx.x - 1) / per;
+    const int first = (int)((blockIdx.x - 1) % per * (256 * kUnroll) + threadIdx.x);
+    const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
+    Raw raw[kUnroll];
+#pragma unroll
+    for (int q = 0; q < kUnroll; q++) raw[q] = load_row<true>(z, (first + q * 256) * N, a.C, (int)a.ldl);   // (past the row: reads nothing)
+    const MaxSum row = join_parts(parts + r * kSplits);
+    const PolicyInputs x = policy_inputs(p, r);
+    const long long lab = a.labels[r];
+    const bool used = lab >= 0 && lab < a.C && x.w != 0.f;
+    float f = 0.f, lp;
+    bool near = false;
+    PolicyTerms none = {0, 0, 0, 0};
+    if (used) f = policy_of_row(p, x, (float)z[lab], row, false, lp, near, none);
+    if (near) f = policy_of_exact(p, x, exact_logp((float)z[lab], row.m, block_sum_f64(exact_part(z, a.C, row.m, threadIdx.x, 256), sh)), false, lp, none);
+    const float fs = f * __builtin_amdgcn_rcpf(row.s);
+#pragma unroll
+    for (int q = 0; q < kUnroll; q++) {
+        const int i = (first + q * 256) * N;
+        if (i >= a.ldl) continue;
+        float v[N];
+        grad_vec<T>(raw[q], row.m, fs, f, used ? (int)lab - i : -1, v);
+        if (f == 0.f) {
+#pragma unroll
+            for (int k = 0; k < N; k++) v[k] = 0.f;
+        }
+        store_row<TD>(dlogits + r * a.ldl, i, (int)a.ldl, v, false);
     }
 }
 
@@ -763,16 +813,17 @@ bool launch_block(const Rows &a, const Policy &p, const Outputs &out, int cap, i
 #undef EMADAPT_BLOCK
     return true;
 }
-inline int stats_width(int C) { return C <= 16384 ? 4 : 16; }   // waves to a row
+// Waves to a row: 16 where the row fills a round of their loads, enough in flight for a CU's share of the memory's rate (bf16, with 4 waves and with
+// 16: 4000 x 27000 33.7 and 38.8 us, 4001 x 32768 with the gradient behind it 126.6 and 122.5, 2000 x 65536 42.6 and 39.9).
+template <typename T> int stats_width(int C) { return C < 16 * 64 * 4 * Vec<T>::N ? 4 : 16; }
 // again: the rows are read once more afterwards
 template <typename T>
 int launch_stats_t(Rows a, const Outputs &out, int splits, bool again, hipStream_t stream) {
     int blocks;
     a.last = !again;
     if (splits > 1 || !launch_short<kLogp, T, T>(a, Policy(), out, 1 << 16, &blocks, stream)) {
-        // a workgroup wide enough to hold what a CU's share of the memory's rate needs in flight (rows of 32768 bf16: 95 us with 16 waves, 102 with 4)
         const dim3 grid(grid_of(a.M, 1 << 16), splits);
-        const bool narrow = splits > 1 || stats_width(a.C) == 4;
+        const bool narrow = splits > 1 || stats_width<T>(a.C) == 4;
         if (narrow && again) hipLaunchKernelGGL((stream_stats_kernel<T, 4, false>), grid, dim3(256), 0, stream, a, out);
         else if (narrow) hipLaunchKernelGGL((stream_stats_kernel<T, 4, true>), grid, dim3(256), 0, stream, a, out);
         else if (again) hipLaunchKernelGGL((stream_stats_kernel<T, 16, false>), grid, dim3(1024), 0, stream, a, out);
@@ -821,7 +872,7 @@ struct PolicySpace {
     unsigned char *near;        // [M]
     size_t bytes;
 };
-constexpr int64_t kFewRows = 128;
+constexpr int64_t kFewRows = 128;   // (33000 bf16: 128 rows 16.3 us in parts, 17 with a workgroup to a row; 192 rows 22.7 and 15.6)
 PolicySpace policy_space(void *workspace, int64_t M) {
     PolicySpace s;
     size_t at = 0;
@@ -840,6 +891,16 @@ PolicySpace policy_space(void *workspace, int64_t M) {
     s.near = reinterpret_cast<unsigned char *>(take((size_t)M));
     s.bytes = at;
     return s;
+}
+
+template <typename T, typename TD>
+int launch_few(const Rows &a, const Policy &p, const MaxSum *parts, float *logp, float *sums, TD *d, hipStream_t stream) {
+    const int64_t nvec = ceil_div(a.ldl, Vec<T>::N);
+    const bool four = nvec * a.M >= 4 * 256 * 1024;   // (as in launch_grad_t)
+    const unsigned per = (unsigned)ceil_div(nvec, four ? 1024 : 256), blocks = d ? 1 + (unsigned)a.M * per : 1;
+    if (four) hipLaunchKernelGGL((policy_few_kernel<T, TD, 4>), dim3(blocks), dim3(256), 0, stream, a, p, parts, logp, sums, d, per);
+    else hipLaunchKernelGGL((policy_few_kernel<T, TD, 1>), dim3(blocks), dim3(256), 0, stream, a, p, parts, logp, sums, d, per);
+    return launch_status();
 }
 
 template <typename T, typename TD>
@@ -868,12 +929,13 @@ int policy_t(Rows a, Policy p, float *sums, float *logp, void *dlogits, int ddt,
         if (int rc = launch_status()) return rc;
         if (!done) {   // rows that no workgroup's registers hold, that are only read, or too few: log-sum-exp, the rows' terms, the gradient
             Outputs st = {};
-            p.tol = border_tol((int)ceil_div(a.C, few ? kSplits * 256 * Vec<T>::N : stats_width(a.C) * 64 * Vec<T>::N) + (few ? kSplits : 0), (int)a.C);
+            p.tol = border_tol((int)ceil_div(a.C, few ? kSplits * 256 * Vec<T>::N : stats_width<T>(a.C) * 64 * Vec<T>::N) + (few ? kSplits : 0), (int)a.C);
             if (few) st.parts = w.parts;
             else { st.base = w.base; st.sum = w.sum; }
             if (int rc = launch_stats_t<T>(a, st, few ? kSplits : 1, dlogits != nullptr, stream)) return rc;
+            if (few) return launch_few<T, TD>(a, p, w.parts, logp, sums, static_cast<TD *>(dlogits), stream);
             blocks = (int)grid_of(ceil_div(a.M, 256), kPolicyBlocks);
-            hipLaunchKernelGGL(policy_row_kernel<T>, dim3(blocks), dim3(256), 0, stream, a, p, st.parts, w.base, w.sum, logp, w.coef, w.partial, sums);
+            hipLaunchKernelGGL(policy_row_kernel<T>, dim3(blocks), dim3(256), 0, stream, a, p, w.base, w.sum, logp, w.coef, w.partial, sums);
             if (int rc = launch_status()) return rc;
             if (dlogits)
                 if (int rc = launch_grad_t<T>(a, w.base, w.sum, w.coef, dlogits, ddt, stream)) return rc;
@@ -899,7 +961,7 @@ int emadapt_label_logp(const void *logits, int dtype, int64_t ldl, const int64_t
     hipStream_t stream = as_stream(stream_);
     ProfScope prof(EMADAPT_K_OTHER, 0.0, (double)M * ((double)C * dt_size(dtype) + 16.0), stream);
     // (whether a gradient follows is not known here: of up to twice the cache a second reader still finds a good part -- 4001 x 32768 bf16 with
-    // the gradient 127 us, 138 where the first reader leaves nothing; 1500 x 100003 f32 alone 98 and 92)
+    // the gradient 123 us, 140 where the first reader leaves nothing; 1500 x 100003 f32 alone 100 and 92)
     const bool again = (double)M * C * dt_size(dtype) < 2 * kCache;
     return launch_stats(rows_of(logits, ldl, labels, M, C), dtype, Outputs{logp, lse}, again, stream);
 }
