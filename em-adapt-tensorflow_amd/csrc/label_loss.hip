@@ -315,7 +315,9 @@ __device__ __forceinline__ float policy_of_exact(const Policy &p, const PolicyIn
 }
 
 // L lanes to a row, NV vectors of the padded row to a lane: few lanes, so that what is done once a row (logarithm, loss) is done for many rows by
-// a wave's instruction (1.6 M rows of 24 f32: 54 us with a vector to a lane, 39 with three).
+// a wave's instruction (1.6 M rows of 24 f32: 54 us with a vector to a lane, 39 with three).  One pass: logits in, and with the policy loss their
+// gradient out; HBM bounds it from some 100000 rows on (logp of those rows 28.6 us in the kernel, 5.8 TB/s; 195312 rows of 1024 f32 65 us, 6.1),
+// below that the launches.  Policy: 64-bit logarithms and differences to each row keep narrow rows at 3 to 4 TB/s.
 template <typename T, typename TD, int L, int NV, int MODE>
 __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs out) {
     constexpr int N = Vec<T>::N;
@@ -323,6 +325,7 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
     const int lane = threadIdx.x % L;
     const long long per_grid = (long long)gridDim.x * (256 / L);
     PolicyTerms t = {0, 0, 0, 0};
+    if (MODE != kLogp && blockIdx.x == 0 && threadIdx.x == 0) *out.ticket = 0u;
     for (long long r = (long long)blockIdx.x * (256 / L) + threadIdx.x / L; r < a.M; r += per_grid) {
         const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
         const long long lab = a.labels[r];
@@ -364,16 +367,11 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
         }
         s = group_sum<L>(s);
         float lp = 0.f, f = 0.f;
+        bool near = false;
         if (used) {
             if (MODE == kLogp) lp = (float)logp_of(zl, MaxSum{m, s});
             else {
-                bool near;
                 f = policy_of_row(p, x, zl, MaxSum{m, s}, lane == 0, lp, near, t);
-                if (near) {
-                    double e = exact_part(z, a.C, m, lane, L);
-                    for (int o = L / 2; o > 0; o >>= 1) e += __shfl_xor(e, o);
-                    f = policy_of_exact(p, x, exact_logp(zl, m, e), lane == 0, lp, t);
-                }
             }
         }
         if (lane == 0) {
@@ -382,6 +380,9 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
                 if (out.lse) out.lse[r] = m + logf(s);
                 if (out.base) { out.base[r] = m; out.sum[r] = s; }
                 if (out.zero) out.zero[r] = 0.f;
+            } else {   // (rows near a border: policy_finish_kernel's -- their 64-bit exponentials here would double the registers of all rows)
+                out.near[r] = near;
+                if (near) out.base[r] = m;
             }
         }
         if (MODE == kPolicyGrad) {
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
 #pragma unroll
                     for (int e = 0; e < N; e++) v[e] = 0.f;
                 }
-                store_row<TD>(static_cast<TD *>(out.dlogits) + r * a.ldl, i, (int)a.ldl, v, a.once);
+                store_row<TD>(static_cast<TD *>(out.dlogits) + r * a.ldl, i, (int)a.ldl, v, a.once && L >= 32);
             }
         }
     }
@@ -427,7 +428,9 @@ template <int N> __device__ __forceinline__ void take(const float (&v)[N], float
     m = top;
 }
 
-// A workgroup of W waves to a row, NV whole vectors to a thread, and the C % N last elements one to a thread.
+// A workgroup of W waves to a row, NV whole vectors to a thread, and the C % N last elements one to a thread.  HBM bounds it, each logit read and
+// each gradient written once: 4096 x 65536 bf16 199 us, 5.4 TB/s of the 4.8 to 5.3 that a copy of that size reaches (330 us where statistics and
+// gradient each read the logits).
 template <typename T, typename TD, int W, int NV, int MODE>
 __global__ void __launch_bounds__(64 * W, 4) block_kernel(Rows a, Policy p, Outputs out) {
     constexpr int N = Vec<T>::N, kThreads = 64 * W;
@@ -512,7 +515,8 @@ __global__ void __launch_bounds__(64 * W, 4) block_kernel(Rows a, Policy p, Outp
     }
 }
 
-// One workgroup to a row of any length, read once: a running maximum and sum for every thread, kAhead vectors in flight.
+// One workgroup to a row of any length, read once: a running maximum and sum for every thread, kAhead vectors in flight.  Bound by HBM: 1500 x 100003
+// f32 90 us in the kernel, 6.65 TB/s.
 template <typename T, int W, bool ONCE>
 __global__ void __launch_bounds__(64 * W) stream_stats_kernel(Rows a, Outputs out) {
     constexpr int N = Vec<T>::N, kThreads = 64 * W, kAhead = 4;
@@ -661,7 +665,8 @@ __global__ void __launch_bounds__(256) policy_few_kernel(Rows a, Policy p, const
     }
 }
 
-// The sums of the launch before, and its rows near a border (near, or null) in 64 bits: 1024 rows to a workgroup, nearly all of which find none.
+constexpr int kFinishRows = 16 * 1024;   // to a workgroup
+// The sums of the launch before, and its rows near a border (near, or null) in 64 bits: most workgroups find none.
 // Their terms were left out there; logp and the gradient are written again.  The last workgroup adds everything up in a fixed order.
 template <typename T, typename TD>
 __global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, Outputs out, int nparts, double *__restrict__ fixed, float *__restrict__ sums) {
@@ -671,26 +676,40 @@ __global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, O
     __shared__ bool last;
     PolicyTerms t = {0, 0, 0, 0};
     if (out.near) {
-        const long long r0 = (long long)blockIdx.x * 1024, mine = r0 + threadIdx.x;
-        const unsigned long long b = __ballot(mine < a.M && out.near[mine]);
-        if ((threadIdx.x & 63) == 0) mask[threadIdx.x >> 6] = b;
-        __syncthreads();
-        for (int q = 0; q < 16; q++)
-            for (unsigned long long left = mask[q]; left; left &= left - 1) {
-                const long long r = r0 + q * 64 + (__ffsll((long long)left) - 1), lab = a.labels[r];
-                const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
-                const float top = out.base[r];
-                const double sum = block_sum_f64(exact_part(z, a.C, top, threadIdx.x, 1024), one), lp64 = exact_logp((float)z[lab], top, sum);
-                float lp;
-                const float f = policy_of_exact(p, policy_inputs(p, r), lp64, threadIdx.x == 0, lp, t);
-                if (threadIdx.x == 0) out.logp[r] = lp;
-                if (!out.dlogits) continue;
-                TD *d = static_cast<TD *>(out.dlogits) + r * a.ldl;
-                const float over = (float)((double)f / sum);
-#pragma unroll 1
-                for (int i = threadIdx.x; i < a.C; i += 1024)
-                    d[i] = (TD)(f == 0.f ? 0.f : (i == (int)lab ? f : 0.f) - __expf((float)z[i] - top) * over);
+        // 16 rows to a thread at a look, and 1024 to the workgroup where there are any
+        for (long long r0 = (long long)blockIdx.x * kFinishRows, look = r0; r0 < a.M; r0 = look) {
+            if (r0 % kFinishRows == 0) {
+                const long long at = r0 + threadIdx.x * 16;
+                const Raw some = at < a.M ? *reinterpret_cast<const Raw *>(out.near + at) : Raw{0, 0, 0, 0};
+                if (!__syncthreads_or(some[0] | some[1] | some[2] | some[3])) {
+                    look = r0 + (long long)gridDim.x * kFinishRows;
+                    continue;
+                }
             }
+            look = r0 + 1024;
+            if (look % kFinishRows == 0) look += (long long)(gridDim.x - 1) * kFinishRows;
+            const long long mine = r0 + threadIdx.x;
+            const unsigned long long b = __ballot(mine < a.M && out.near[mine]);
+            if ((threadIdx.x & 63) == 0) mask[threadIdx.x >> 6] = b;
+            __syncthreads();
+            for (int q = 0; q < 16; q++)
+                for (unsigned long long left = mask[q]; left; left &= left - 1) {
+                    const long long r = r0 + q * 64 + (__ffsll((long long)left) - 1), lab = a.labels[r];
+                    const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
+                    const float top = out.base[r];
+                    const double sum = block_sum_f64(exact_part(z, a.C, top, threadIdx.x, 1024), one), lp64 = exact_logp((float)z[lab], top, sum);
+                    float lp;
+                    const float f = policy_of_exact(p, policy_inputs(p, r), lp64, threadIdx.x == 0, lp, t);
+                    if (threadIdx.x == 0) out.logp[r] = lp;
+                    if (!out.dlogits) continue;
+                    TD *d = static_cast<TD *>(out.dlogits) + r * a.ldl;
+                    const float over = (float)((double)f / sum);
+#pragma unroll 1
+                    for (int i = threadIdx.x; i < a.C; i += 1024)
+                        d[i] = (TD)(f == 0.f ? 0.f : (i == (int)lab ? f : 0.f) - __expf((float)z[i] - top) * over);
+                }
+            __syncthreads();
+        }
         // (a ticket among few workgroups; the part is where every CU sees it before the ticket counts it)
         if (threadIdx.x == 0) {
             const double s[4] = {t.loss, t.surrogate, t.kl, t.clipped};
@@ -720,35 +739,66 @@ __global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, O
 }
 
 // ------------------------------------------------------------------------------------------
-// the preference loss: one workgroup to a pair of sequences
+// the preference loss: one workgroup to a pair of sequences, or (SPLIT) gridDim.x of them where pairs are long
 // ------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(1024) preference_pair_kernel(const float *__restrict__ logp, const long long *__restrict__ seq_start, const float *__restrict__ ref,
-                                                             long long M, float beta, float smooth, float scale, float *__restrict__ loss,
-                                                             float *__restrict__ seq_logp, float *__restrict__ coef) {
+struct Preference {
+    const float *logp;
+    const long long *seq_start;
+    const float *ref;
+    long long M;
+    float beta, smooth, scale;
+    float *loss, *seq_logp, *coef;   // coef: or null
+    double *part;                    // SPLIT: [2 pairs][gridDim.x] sums of parts of the sequences
+};
+// rows of part x of n of sequence s (a start outside the rows, or before the one in front of it, reads and writes nothing)
+__device__ __forceinline__ void part_of(const Preference &a, long long s, unsigned x, unsigned n, long long &begin, long long &end) {
+    const long long lo = min(max(a.seq_start[s], 0ll), a.M), hi = min(max(a.seq_start[s + 1], 0ll), a.M), per = hi > lo ? (hi - lo + n - 1) / n : 0;
+    begin = lo + x * per;
+    end = min(begin + per, hi);
+}
+__device__ __forceinline__ double part_sum(const Preference &a, long long begin, long long end, double *sh) {
+    double v = 0.0;
+    for (long long r = begin + threadIdx.x; r < end; r += 1024) v += (double)a.logp[r];
+    return block_sum_f64(v, sh);
+}
+__global__ void __launch_bounds__(1024) preference_part_kernel(Preference a) {   // sequence blockIdx.y
     __shared__ double sh[16];
-    const long long pair = blockIdx.x;
-    long long at[3];
-    for (int k = 0; k < 3; k++) {   // (a start outside the rows, or before the one in front of it, reads and writes nothing)
-        const long long v = seq_start[2 * pair + k];
-        at[k] = v < 0 ? 0 : (v > M ? M : v);
-    }
+    long long begin, end;
+    part_of(a, blockIdx.y, blockIdx.x, gridDim.x, begin, end);
+    const double v = part_sum(a, begin, end, sh);
+    if (threadIdx.x == 0) a.part[(long long)blockIdx.y * gridDim.x + blockIdx.x] = v;
+}
+template <bool SPLIT> __global__ void __launch_bounds__(1024) preference_pair_kernel(Preference a) {
+    __shared__ double sh[16];
+    const long long pair = SPLIT ? blockIdx.y : blockIdx.x;
+    const unsigned x = SPLIT ? blockIdx.x : 0, n = SPLIT ? gridDim.x : 1;
+    long long begin[2], end[2];
     double s[2];
     for (int q = 0; q < 2; q++) {
-        double v = 0.0;
-        for (long long r = at[q] + threadIdx.x; r < at[q + 1]; r += 1024) v += (double)logp[r];
-        s[q] = block_sum_f64(v, sh);
+        part_of(a, 2 * pair + q, x, n, begin[q], end[q]);
+        if (SPLIT) {
+            double v = 0.0;
+            for (unsigned i = threadIdx.x; i < n; i += 1024) v += a.part[(2 * pair + q) * n + i];
+            s[q] = block_sum_f64(v, sh);
+        } else s[q] = part_sum(a, begin[q], end[q], sh);
     }
-    const double h = (double)beta * ((s[0] - (double)ref[2 * pair]) - (s[1] - (double)ref[2 * pair + 1]));
-    const double soft = log1p(exp(-fabs(h)));   // softplus(h) = soft + max(h, 0)
-    if (threadIdx.x == 0) {
-        loss[pair] = (float)((1.0 - (double)smooth) * (soft - fmin(h, 0.0)) + (double)smooth * (soft + fmax(h, 0.0)));
-        seq_logp[2 * pair] = (float)s[0];
-        seq_logp[2 * pair + 1] = (float)s[1];
+    const double h = (double)a.beta * ((s[0] - (double)a.ref[2 * pair]) - (s[1] - (double)a.ref[2 * pair + 1]));
+    if (threadIdx.x == 0 && x == 0) {
+        const double soft = log1p(exp(-fabs(h)));   // softplus(h) = soft + max(h, 0)
+        a.loss[pair] = (float)((1.0 - (double)a.smooth) * (soft - fmin(h, 0.0)) + (double)a.smooth * (soft + fmax(h, 0.0)));
+        a.seq_logp[2 * pair] = (float)s[0];
+        a.seq_logp[2 * pair + 1] = (float)s[1];
     }
-    if (!coef) return;
-    const float g = (float)((double)scale * (double)beta * ((double)smooth - 1.0 / (1.0 + exp(h))));
+    if (!a.coef) return;
+    const float g = (float)((double)a.scale * (double)a.beta * ((double)a.smooth - 1.0 / (1.0 + exp(h))));
     for (int q = 0; q < 2; q++)
-        for (long long r = at[q] + threadIdx.x; r < at[q + 1]; r += 1024) coef[r] = q ? -g : g;
+        for (long long r = begin[q] + threadIdx.x; r < end[q]; r += 1024) a.coef[r] = q ? -g : g;
+}
+// Parts of a pair: 8192 rows each, where it has 32768 and more on average (all launches of the loss over f32 rows of 24, a workgroup to a pair and
+// parts: 2 pairs of 16384 rows 19.1 us and 21.2, of 32768 21.7 and 21.2, 8 of 206081 154 and 101).
+inline int64_t pair_parts(int64_t M, int64_t pairs) {
+    const int64_t want = M / pairs < 32768 || pairs > 16384 ? 1 : ceil_div(M, pairs * 8192);   // (2 pairs go into a grid's second dimension)
+    return want < 256 ? want : 256;
 }
 inline bool is_dt(int dt) { return dt == EMADAPT_DT_F32 || dt == EMADAPT_DT_BF16; }
 inline size_t dt_size(int dt) { return dt == EMADAPT_DT_BF16 ? 2 : 4; }
@@ -774,13 +824,18 @@ Rows rows_of(const void *logits, int64_t ldl, const int64_t *labels, int64_t M, 
     return Rows{logits, reinterpret_cast<const long long *>(labels), (long long)ldl, (long long)M, (int)C, (double)M * ldl * grad_size > kCache / 4, false};
 }
 
-// Rows of up to 64 vectors, three or four of them to a lane.  false: longer rows.
+// Rows of up to 64 vectors, three or four of them to a lane; up to 8 where that still beats a workgroup to a row.  False: longer rows.
+//   statistics  512 vectors (200 M bf16, rows of 520: 105 us against 375; of 4096: 68 against 84), 384 where nothing is left in the cache (of 4000:
+//               117 against 88)
+//   gradient    384 vectors (rows of 520: 283 us against 688, of 2047 208 against 282, of 2900 202 against 208, of 4000 230 against 170)
+//   loss alone  16 vectors, behind them statistics and rows' terms in two launches (f32 rows of 24: 52 us against 75 for 1.6 M, of 64: 106 against
+//               121, of 130: 135 against 114)
 template <int MODE, typename T, typename TD>
 bool launch_short(const Rows &a, const Policy &p, const Outputs &out, int cap, int *blocks, hipStream_t stream) {
     const int64_t nvec = ceil_div(a.ldl, Vec<T>::N);
-    if (nvec > 64) return false;
+    if (nvec > (MODE == kLogp ? (a.last ? 384 : 512) : MODE == kPolicyGrad ? 384 : 16)) return false;
     int L = 1;
-    while (L * 4 < nvec) L *= 2;
+    while (L * 4 < nvec && L < 64) L *= 2;
     const bool three = nvec <= 3 * L;
     *blocks = (int)grid_of(ceil_div(a.M, 256 / L), cap);
 #define EMADAPT_GROUP(L, NV) hipLaunchKernelGGL((group_kernel<T, TD, L, NV, MODE>), dim3(*blocks), dim3(256), 0, stream, a, p, out)
@@ -788,8 +843,16 @@ bool launch_short(const Rows &a, const Policy &p, const Outputs &out, int cap, i
         case 1: if (three) EMADAPT_GROUP(1, 3); else EMADAPT_GROUP(1, 4); break;
         case 2: if (three) EMADAPT_GROUP(2, 3); else EMADAPT_GROUP(2, 4); break;
         case 4: if (three) EMADAPT_GROUP(4, 3); else EMADAPT_GROUP(4, 4); break;
+    }
+    if constexpr (MODE != kPolicy) switch (L) {
         case 8: if (three) EMADAPT_GROUP(8, 3); else EMADAPT_GROUP(8, 4); break;
-        default: if (three) EMADAPT_GROUP(16, 3); else EMADAPT_GROUP(16, 4);
+        case 16: if (three) EMADAPT_GROUP(16, 3); else EMADAPT_GROUP(16, 4); break;
+        case 32: if (three) EMADAPT_GROUP(32, 3); else EMADAPT_GROUP(32, 4); break;
+        case 64:
+            if (three) EMADAPT_GROUP(64, 3);
+            else if (nvec <= 256) EMADAPT_GROUP(64, 4);
+            else if (nvec <= 384) EMADAPT_GROUP(64, 6);
+            else if constexpr (MODE == kLogp) EMADAPT_GROUP(64, 8);
     }
 #undef EMADAPT_GROUP
     return true;
@@ -861,13 +924,13 @@ int launch_grad_t(const Rows &a, const float *base, const float *sum, const floa
 int launch_grad(const Rows &a, int dtype, const float *base, const float *sum, const float *coef, void *d, int ddt, hipStream_t stream) {
     return dtype == EMADAPT_DT_BF16 ? launch_grad_t<__bf16>(a, base, sum, coef, d, ddt, stream) : launch_grad_t<float>(a, base, sum, coef, d, ddt, stream);
 }
-constexpr int kPolicyBlocks = 2048;
+constexpr int kPolicyBlocks = 2048, kFinishBlocks = 512;
 
 // Where the policy loss keeps what its launches hand on.
 struct PolicySpace {
     float *base, *sum, *coef;   // [M] each
     MaxSum *parts;              // [kFewRows][kSplits]
-    double *partial, *fixed;    // [kPolicyBlocks][4], [ceil(M / 1024)][4]
+    double *partial, *fixed;    // [kPolicyBlocks][4], [kFinishBlocks][4]
     unsigned *ticket;
     unsigned char *near;        // [M]
     size_t bytes;
@@ -886,9 +949,9 @@ PolicySpace policy_space(void *workspace, int64_t M) {
     s.coef = s.sum + M;
     s.parts = reinterpret_cast<MaxSum *>(take(kFewRows * kSplits * sizeof(MaxSum)));
     s.partial = reinterpret_cast<double *>(take((size_t)kPolicyBlocks * 32));
-    s.fixed = reinterpret_cast<double *>(take((size_t)ceil_div(M, 1024) * 32));
+    s.fixed = reinterpret_cast<double *>(take((size_t)kFinishBlocks * 32));
     s.ticket = reinterpret_cast<unsigned *>(take(4));
-    s.near = reinterpret_cast<unsigned char *>(take((size_t)M));
+    s.near = reinterpret_cast<unsigned char *>(take((size_t)M + 16));   // (looked at 16 at a time)
     s.bytes = at;
     return s;
 }
@@ -915,17 +978,15 @@ int policy_t(Rows a, Policy p, float *sums, float *logp, void *dlogits, int ddt,
         bool done;
         a.last = a.once;
         p.tol = border_tol(16, (int)a.C);   // (short rows: none; a row in registers: 16 vectors to a thread)
+        out.near = w.near;
+        out.base = w.base;
         if (!dlogits) done = launch_short<kPolicy, T, T>(a, p, out, kPolicyBlocks, &blocks, stream);
         else {
             done = launch_short<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
-            if (!done && !few) {
-                out.near = w.near;
-                out.base = w.base;
-                done = launch_block<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
-                if (done) finish = (unsigned)ceil_div(a.M, 1024);
-                else out.near = nullptr;
-            }
+            if (!done && !few) done = launch_block<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
         }
+        if (done) finish = grid_of(ceil_div(a.M, kFinishRows), kFinishBlocks);
+        else out.near = nullptr;
         if (int rc = launch_status()) return rc;
         if (!done) {   // rows that no workgroup's registers hold, that are only read, or too few: log-sum-exp, the rows' terms, the gradient
             Outputs st = {};
@@ -998,7 +1059,9 @@ int emadapt_policy_loss(const void *logits, int dtype, int64_t ldl, const int64_
 
 size_t emadapt_preference_loss_workspace_bytes(int64_t M, int64_t C) {
     (void)C;
-    return (size_t)(M > 0 ? M : 1) * 16;
+    // (four floats a row; parts of long pairs: at most M / 8192 + pairs of them, pairs <= M / 32768, two sums each)
+    const size_t rows = M > 0 ? (size_t)M : 1;
+    return align_up(rows * 16, 256) + rows / 8192 * 24 + 64;
 }
 
 int emadapt_preference_loss(const void *logits, int dtype, int64_t ldl, const int64_t *labels, const int64_t *seq_start, int64_t pairs, const float *ref_logp,
@@ -1008,7 +1071,7 @@ int emadapt_preference_loss(const void *logits, int dtype, int64_t ldl, const in
     if (pairs < 0 || !(label_smoothing >= 0.f && label_smoothing <= 1.f) || !isfinite(beta) || !isfinite(grad_scale)) return EMADAPT_ERR_INVALID;
     if (pairs > 0x7FFFFFFF) return EMADAPT_ERR_UNSUPPORTED;
     if (pairs && (!seq_start || !aligned(seq_start, 8) || !ref_logp || !loss || !seq_logp)) return EMADAPT_ERR_INVALID;
-    if (M && (!workspace || !aligned(workspace, 4) || workspace_bytes < emadapt_preference_loss_workspace_bytes(M, C))) return EMADAPT_ERR_WORKSPACE;
+    if (M && (!workspace || !aligned(workspace, 8) || workspace_bytes < emadapt_preference_loss_workspace_bytes(M, C))) return EMADAPT_ERR_WORKSPACE;
     hipStream_t stream = as_stream(stream_);
     ProfScope prof(EMADAPT_K_OTHER, 0.0, (double)M * (2.0 * C * dt_size(dtype) + (dlogits ? (double)ldl * dt_size(dlogits_dtype) : 0.0) + 24.0), stream);
     float *logp = static_cast<float *>(workspace), *base = logp + M, *sum = base + M, *coef = sum + M;
@@ -1016,8 +1079,14 @@ int emadapt_preference_loss(const void *logits, int dtype, int64_t ldl, const in
     if (M)   // (rows of no sequence have no gradient: their coefficient starts at 0)
         if (int rc = launch_stats(a, dtype, Outputs{logp, nullptr, dlogits ? base : nullptr, sum, dlogits ? coef : nullptr}, dlogits != nullptr, stream)) return rc;
     if (pairs) {
-        hipLaunchKernelGGL(preference_pair_kernel, dim3((unsigned)pairs), dim3(1024), 0, stream, logp, reinterpret_cast<const long long *>(seq_start), ref_logp, (long long)M,
-                           beta, label_smoothing, grad_scale, loss, seq_logp, dlogits ? coef : nullptr);
+        const Preference p = {logp, reinterpret_cast<const long long *>(seq_start), ref_logp, (long long)M, beta, label_smoothing, grad_scale, loss, seq_logp,
+                              dlogits ? coef : nullptr, reinterpret_cast<double *>(static_cast<char *>(workspace) + align_up((size_t)M * 16, 256))};
+        const int64_t parts = pair_parts(M, pairs);
+        if (parts > 1) {
+            hipLaunchKernelGGL(preference_part_kernel, dim3((unsigned)parts, (unsigned)(2 * pairs)), dim3(1024), 0, stream, p);
+            hipLaunchKernelGGL(preference_pair_kernel<true>, dim3((unsigned)parts, (unsigned)pairs), dim3(1024), 0, stream, p);
+        } else
+            hipLaunchKernelGGL(preference_pair_kernel<false>, dim3((unsigned)pairs), dim3(1024), 0, stream, p);
         if (int rc = launch_status()) return rc;
     }
     if (M && dlogits) return launch_grad(a, dtype, base, sum, coef, dlogits, dlogits_dtype, stream);

@@ -240,7 +240,7 @@ def test_policy_loss(env, shape, dtype):
         assert bool(((logp2.double() - want_lp).abs() <= torch.where(used, lp_tol, torch.zeros_like(lp_tol))).all())
 
 
-@pytest.mark.parametrize("shape", [(4000, 21, 24), (300, 700, 700), (64, 40000, 40000), (5, 150001, 150001)])
+@pytest.mark.parametrize("shape", [(4000, 21, 24), (300, 700, 700), (64, 40000, 40000), (5, 150001, 150001), (70001, 5, 5), (40000, 130, 130), (600, 5000, 5000)])
 def test_policy_clip_is_decided_as_in_64_bits(env, shape):
     """old_logp such that the ratio lies a few f32 roundings to either side of a border, nearer than f32 can tell."""
     ops, torch = env
@@ -523,3 +523,29 @@ def test_kl_of_weight_zero_does_not_count(env):
         a = ops.policy_loss(z, lab, logp - 0.05, adv, C, kl_coef=0.0)
         b = ops.policy_loss(z, lab, logp - 0.05, adv, C, ref_logp=logp + 120.0, kl_coef=0.0)   # exp(120) is beyond f32
         assert torch.equal(a[0][:2], b[0][:2]) and torch.equal(a[2], b[2]) and bool(torch.isfinite(b[2]).all())
+
+
+def test_preference_of_long_sequences(env):
+    """Pairs long enough to be split over workgroups, of unlike lengths, an empty sequence among them, rows of no sequence in front and behind."""
+    ops, torch = env
+    C = 5
+    lens = [40000, 25001, 0, 70003, 1, 8192]
+    M = sum(lens) + 30
+    z = _logits(torch, M, C, "float32", 12)
+    lab = _labels(torch, M, C, 12)
+    at = torch.tensor(10 + np.concatenate([[0], np.cumsum(lens)]), device="cuda")
+    true = _preference_reference(torch, z, lab, at, torch.zeros(6, device="cuda"), C, 0.1, 0.0, 1.0)[4]
+    ref = (true + torch.tensor([1.0, -1.0, 2.0, 3.0, -4.0, 0.5], device="cuda")).float()
+    loss, seq, d = ops.preference_loss(z, lab, at, ref, C, beta=0.2, label_smoothing=0.1, grad_scale=1.0, dlogits=torch.full_like(z, 3.0))
+    x, lse, used, tol, wseq, seq_tol, wloss, loss_tol, coef, coef_tol = _preference_reference(torch, z, lab, at, ref, C, 0.2, 0.1, 1.0)
+    assert bool(((seq.double() - wseq).abs() <= seq_tol).all()) and bool(((loss.double() - wloss).abs() <= loss_tol).all())
+    _check_grad(torch, d, x, lse, used, lab, coef, coef_tol, tol, C)
+    assert bool((d[:10] == 0).all()) and bool((d[M - 20:] == 0).all())
+    again = ops.preference_loss(z, lab, at, ref, C, beta=0.2, label_smoothing=0.1, grad_scale=1.0)
+    assert torch.equal(again[0], loss) and torch.equal(again[2], d)
+    # starts out of range and out of order: nothing outside the rows is touched
+    room = torch.full((M + 20, C), 5.0, device="cuda")
+    for starts in ([0, 2 ** 40, 2 ** 41], [-9, 50000, 20], [M + 5, M + 9, M + 12]):
+        ops.preference_loss(z, lab, torch.tensor(starts, device="cuda"), ref[:2].contiguous(), C, dlogits=room[10:M + 10])
+        torch.cuda.synchronize()
+        assert bool((room[:10] == 5).all()) and bool((room[M + 10:] == 5).all())
