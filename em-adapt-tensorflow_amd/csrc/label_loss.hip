@@ -270,12 +270,22 @@ __device__ __forceinline__ bool near_border(double log_ratio, float adv, const P
     const double border = adv > 0.f ? p.log_high : p.log_low;
     return adv != 0.f && fabs(log_ratio - border) < (double)p.tol;
 }
-// sum over elements `first`, first + step, .. of the row of exp(z - its maximum) in 64 bits; the label's log-probability from the whole sum
-template <typename T>
+// sum over elements `first`, first + step, .. of the row of exp(z - its maximum) in 64 bits; the label's log-probability from the whole sum.
+// LONG: four loads in flight (one workgroup's way through the row is all that such a row costs), for registers that short rows had better keep.
+template <bool LONG, typename T>
 __device__ double exact_part(const T *z, int C, float top, int first, int step) {
     double s = 0.0;
+    int i = first;
 #pragma unroll 1
-    for (int i = first; i < C; i += step) s += exp((double)(float)z[i] - (double)top);
+    for (; LONG && i + 3 * step < C; i += 4 * step) {
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = (float)z[i + k * step];
+#pragma unroll
+        for (int k = 0; k < 4; k++) s += exp((double)v[k] - (double)top);
+    }
+#pragma unroll 1
+    for (; i < C; i += step) s += exp((double)(float)z[i] - (double)top);
     return s;
 }
 __device__ __forceinline__ double exact_logp(float z, float top, double sum) { return ((double)z - (double)top) - log(sum); }
@@ -314,6 +324,7 @@ __device__ __forceinline__ float policy_of_exact(const Policy &p, const PolicyIn
     return policy_row((float)lr, (float)((double)x.refp - lp64), x.has_ref, x.adv, x.w, p, past_border(lr, x.adv, p), count, t);
 }
 
+constexpr int kInlineLanes = 16;
 // L lanes to a row, NV vectors of the padded row to a lane: few lanes, so that what is done once a row (logarithm, loss) is done for many rows by
 // a wave's instruction (1.6 M rows of 24 f32: 54 us with a vector to a lane, 39 with three).  One pass: logits in, and with the policy loss their
 // gradient out; HBM bounds it from some 100000 rows on (logp of those rows 28.6 us in the kernel, 5.8 TB/s; 195312 rows of 1024 f32 65 us, 6.1),
@@ -321,11 +332,14 @@ __device__ __forceinline__ float policy_of_exact(const Policy &p, const PolicyIn
 template <typename T, typename TD, int L, int NV, int MODE>
 __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs out) {
     constexpr int N = Vec<T>::N;
+    // Rows near a border here, or in policy_finish_kernel: 64-bit exponentials here double the registers of all rows (200 M bf16 in rows of 1000: 252 us
+    // and 198), but find the row's inputs at hand (26896 rows of 24 f32, two of them near a border: 10.8 us and 20.5)
+    constexpr bool kInline = L <= kInlineLanes;
     __shared__ double sh[4];
     const int lane = threadIdx.x % L;
     const long long per_grid = (long long)gridDim.x * (256 / L);
     PolicyTerms t = {0, 0, 0, 0};
-    if (MODE != kLogp && blockIdx.x == 0 && threadIdx.x == 0) *out.ticket = 0u;
+    if (MODE != kLogp && !kInline && blockIdx.x == 0 && threadIdx.x == 0) *out.ticket = 0u;
     for (long long r = (long long)blockIdx.x * (256 / L) + threadIdx.x / L; r < a.M; r += per_grid) {
         const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
         const long long lab = a.labels[r];
@@ -372,6 +386,11 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
             if (MODE == kLogp) lp = (float)logp_of(zl, MaxSum{m, s});
             else {
                 f = policy_of_row(p, x, zl, MaxSum{m, s}, lane == 0, lp, near, t);
+                if (kInline && near) {
+                    double e = exact_part<false>(z, a.C, m, lane, L);
+                    for (int o = L / 2; o > 0; o >>= 1) e += __shfl_xor(e, o);
+                    f = policy_of_exact(p, x, exact_logp(zl, m, e), lane == 0, lp, t);
+                }
             }
         }
         if (lane == 0) {
@@ -380,7 +399,7 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
                 if (out.lse) out.lse[r] = m + logf(s);
                 if (out.base) { out.base[r] = m; out.sum[r] = s; }
                 if (out.zero) out.zero[r] = 0.f;
-            } else {   // (rows near a border: policy_finish_kernel's -- their 64-bit exponentials here would double the registers of all rows)
+            } else if (!kInline) {
                 out.near[r] = near;
                 if (near) out.base[r] = m;
             }
@@ -599,7 +618,7 @@ __device__ void policy_rows(const Rows &a, const Policy &p, const MaxSum *__rest
                 const long long rr = r0 + k;
                 const T *z = static_cast<const T *>(a.logits) + rr * a.ldl;
                 const float top = PARTS ? whole[k].m : base[rr];
-                const double lp64 = exact_logp((float)z[a.labels[rr]], top, block_sum_f64(exact_part(z, a.C, top, threadIdx.x, 256), sh));
+                const double lp64 = exact_logp((float)z[a.labels[rr]], top, block_sum_f64(exact_part<true>(z, a.C, top, threadIdx.x, 256), sh));
                 if (threadIdx.x == 0) {
                     float lp;
                     const float f = policy_of_exact(p, policy_inputs(p, rr), lp64, true, lp, t);
@@ -649,7 +668,7 @@ __global__ void __launch_bounds__(256) policy_few_kernel(Rows a, Policy p, const
     bool near = false;
     PolicyTerms none = {0, 0, 0, 0};
     if (used) f = policy_of_row(p, x, (float)z[lab], row, false, lp, near, none);
-    if (near) f = policy_of_exact(p, x, exact_logp((float)z[lab], row.m, block_sum_f64(exact_part(z, a.C, row.m, threadIdx.x, 256), sh)), false, lp, none);
+    if (near) f = policy_of_exact(p, x, exact_logp((float)z[lab], row.m, block_sum_f64(exact_part<true>(z, a.C, row.m, threadIdx.x, 256), sh)), false, lp, none);
     const float fs = f * __builtin_amdgcn_rcpf(row.s);
 #pragma unroll
     for (int q = 0; q < kUnroll; q++) {
@@ -675,6 +694,7 @@ __global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, O
     __shared__ unsigned long long mask[16];
     __shared__ bool last;
     PolicyTerms t = {0, 0, 0, 0};
+    bool hit = false;
     if (out.near) {
         // 16 rows to a thread at a look, and 1024 to the workgroup where there are any
         for (long long r0 = (long long)blockIdx.x * kFinishRows, look = r0; r0 < a.M; r0 = look) {
@@ -690,30 +710,43 @@ __global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, O
             if (look % kFinishRows == 0) look += (long long)(gridDim.x - 1) * kFinishRows;
             const long long mine = r0 + threadIdx.x;
             const unsigned long long b = __ballot(mine < a.M && out.near[mine]);
+            hit = true;
+            // one row, by `step` threads of which this is number `first`
+            auto exact_row = [&](long long r, int first, int step, auto &&sum_of) {
+                const long long lab = a.labels[r];
+                const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
+                const float top = out.base[r];
+                const double sum = sum_of(exact_part<true>(z, a.C, top, first, step)), lp64 = exact_logp((float)z[lab], top, sum);
+                float lp;
+                const float f = policy_of_exact(p, policy_inputs(p, r), lp64, first == 0, lp, t);
+                if (first == 0) out.logp[r] = lp;
+                if (!out.dlogits) return;
+                TD *d = static_cast<TD *>(out.dlogits) + r * a.ldl;
+                const float over = (float)((double)f / sum);
+#pragma unroll 1
+                for (int i = first; i < a.C; i += step) d[i] = (TD)(f == 0.f ? 0.f : (i == (int)lab ? f : 0.f) - __expf((float)z[i] - top) * over);
+            };
+            if (a.C <= 4096) {   // each wave its own rows
+                for (unsigned long long left = b; left; left &= left - 1)
+                    exact_row(r0 + (threadIdx.x & ~63u) + (__ffsll((long long)left) - 1), threadIdx.x & 63, 64, [](double v) {
+                        for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+                        return v;
+                    });
+                continue;
+            }
             if ((threadIdx.x & 63) == 0) mask[threadIdx.x >> 6] = b;
             __syncthreads();
             for (int q = 0; q < 16; q++)
-                for (unsigned long long left = mask[q]; left; left &= left - 1) {
-                    const long long r = r0 + q * 64 + (__ffsll((long long)left) - 1), lab = a.labels[r];
-                    const T *z = static_cast<const T *>(a.logits) + r * a.ldl;
-                    const float top = out.base[r];
-                    const double sum = block_sum_f64(exact_part(z, a.C, top, threadIdx.x, 1024), one), lp64 = exact_logp((float)z[lab], top, sum);
-                    float lp;
-                    const float f = policy_of_exact(p, policy_inputs(p, r), lp64, threadIdx.x == 0, lp, t);
-                    if (threadIdx.x == 0) out.logp[r] = lp;
-                    if (!out.dlogits) continue;
-                    TD *d = static_cast<TD *>(out.dlogits) + r * a.ldl;
-                    const float over = (float)((double)f / sum);
-#pragma unroll 1
-                    for (int i = threadIdx.x; i < a.C; i += 1024)
-                        d[i] = (TD)(f == 0.f ? 0.f : (i == (int)lab ? f : 0.f) - __expf((float)z[i] - top) * over);
-                }
+                for (unsigned long long left = mask[q]; left; left &= left - 1)
+                    exact_row(r0 + q * 64 + (__ffsll((long long)left) - 1), threadIdx.x, 1024, [&](double v) { return block_sum_f64(v, one); });
             __syncthreads();
         }
+        double own[4] = {t.loss, t.surrogate, t.kl, t.clipped};
+        if (hit)
+            for (int k = 0; k < 4; k++) own[k] = block_sum_f64(own[k], one);
         // (a ticket among few workgroups; the part is where every CU sees it before the ticket counts it)
         if (threadIdx.x == 0) {
-            const double s[4] = {t.loss, t.surrogate, t.kl, t.clipped};
-            for (int k = 0; k < 4; k++) __hip_atomic_store(&fixed[(long long)blockIdx.x * 4 + k], s[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (int k = 0; k < 4; k++) __hip_atomic_store(&fixed[(long long)blockIdx.x * 4 + k], own[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __builtin_amdgcn_s_waitcnt(0);
             last = __hip_atomic_fetch_add(out.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
         }
@@ -827,7 +860,7 @@ Rows rows_of(const void *logits, int64_t ldl, const int64_t *labels, int64_t M, 
 // Rows of up to 64 vectors, three or four of them to a lane; up to 8 where that still beats a workgroup to a row.  False: longer rows.
 //   statistics  512 vectors (200 M bf16, rows of 520: 105 us against 375; of 4096: 68 against 84), 384 where nothing is left in the cache (of 4000:
 //               117 against 88)
-//   gradient    384 vectors (rows of 520: 283 us against 688, of 2047 208 against 282, of 2900 202 against 208, of 4000 230 against 170)
+//   gradient    384 vectors (rows of 520: 278 us against 688, of 2047 217 against 282, of 2900 204 against 208, of 4000 230 against 170)
 //   loss alone  16 vectors, behind them statistics and rows' terms in two launches (f32 rows of 24: 52 us against 75 for 1.6 M, of 64: 106 against
 //               121, of 130: 135 against 114)
 template <int MODE, typename T, typename TD>
@@ -985,7 +1018,7 @@ int policy_t(Rows a, Policy p, float *sums, float *logp, void *dlogits, int ddt,
             done = launch_short<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
             if (!done && !few) done = launch_block<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
         }
-        if (done) finish = grid_of(ceil_div(a.M, kFinishRows), kFinishBlocks);
+        if (done && ceil_div(a.ldl, Vec<T>::N) > kInlineLanes * 4) finish = grid_of(ceil_div(a.M, kFinishRows), kFinishBlocks);
         else out.near = nullptr;
         if (int rc = launch_status()) return rc;
         if (!done) {   // rows that no workgroup's registers hold, that are only read, or too few: log-sum-exp, the rows' terms, the gradient
