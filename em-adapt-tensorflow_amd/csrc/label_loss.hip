@@ -160,7 +160,8 @@ __device__ bool sum_anew(const Rows &a, long long row, bool far, float lse, MaxS
 
 // dz = [c = label] coef - exp(z - base) coef / sum (base, sum: the row's maximum and sum; without SUM base is the log-sum-exp): every thread kUnroll
 // vectors of the flattened [M][vectors per row], all in flight.  A workgroup's vectors lie behind one another; their rows come from one 64-bit
-// division for the workgroup and a 32-bit one for each vector.  Rows far from zero are written again at the end (looked at in front of the store
+// division for the workgroup and a 32-bit one for each vector.  HBM bounds it (4001 x 32768 bf16 behind its statistics 77.5 us, 6.8 TB/s of 4.8 to
+// 6.7 that a copy reaches: a part of the logits is still in the cache).  Rows far from zero are written again at the end (looked at in front of the store
 // they cost the others 4 to 9 % of the time).
 template <typename T, typename TD, int kUnroll, bool SUM>
 __global__ void __launch_bounds__(256) row_grad_kernel(Rows a, const float *__restrict__ base, const float *__restrict__ sum, const float *__restrict__ coef, TD *__restrict__ dlogits,
@@ -772,7 +773,9 @@ __global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, O
 }
 
 // ------------------------------------------------------------------------------------------
-// the preference loss: one workgroup to a pair of sequences, or (SPLIT) gridDim.x of them where pairs are long
+// the preference loss: one workgroup to a pair of sequences, or (SPLIT) gridDim.x of them where pairs are long.  A sequence's sum has to be known
+// before its first gradient, so the logits are read twice around it; the launch itself (6 us for 12 pairs of 3362 rows) waits for its chain of loads,
+// sums and 64-bit exponentials.
 // ------------------------------------------------------------------------------------------
 struct Preference {
     const float *logp;
@@ -898,9 +901,7 @@ bool launch_block(const Rows &a, const Policy &p, const Outputs &out, int cap, i
     *blocks = (int)grid_of(a.M, cap);
     const dim3 grid(*blocks);
 #define EMADAPT_BLOCK(W, NV) hipLaunchKernelGGL((block_kernel<T, TD, W, NV, MODE>), grid, dim3(64 * W), 0, stream, a, p, out)
-    if (nvec <= 128) EMADAPT_BLOCK(1, 2);
-    else if (nvec <= 256) EMADAPT_BLOCK(1, 4);
-    else if (nvec <= 512) EMADAPT_BLOCK(1, 8);
+    if (nvec <= 512) EMADAPT_BLOCK(1, 8);
     else if (nvec <= 1024) EMADAPT_BLOCK(1, 16);
     else if (nvec <= 2048) EMADAPT_BLOCK(2, 16);
     else if (nvec <= 4096) EMADAPT_BLOCK(4, 16);
