@@ -399,3 +399,30 @@ def test_pack_takes_nan_as_zero(env):
     m2, u2 = opt.unpack()
     assert float(m2[3]) == 0 and float(u2[3]) == 0 and float(m2[70]) == 0 and float(u2[70]) == 1
     assert bool(torch.isfinite(m2).all()) and bool(torch.isfinite(u2).all()) and bool((m2[64:70] == 1).all())
+
+
+@pytest.mark.parametrize("state", ["f32", "u8"])
+def test_a_tensor_of_more_than_2_31_elements(env, state):
+    """Elements are worked on one by one (without a norm): the last ones of a large tensor go where they go in a tensor of their own.  (8 bits: the weights,
+    which a first step moves by moments not yet rounded.)"""
+    ops, torch = env
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of free memory")
+    n, tail = 2 ** 31 + 4099, 5000
+    w = torch.empty(n, device="cuda").normal_()
+    g = torch.empty(n, dtype=torch.bfloat16, device="cuda").normal_()
+    ws, gs = w[n - tail:].clone(), g[n - tail:].clone()
+    large, small = ops.AdamW([w], [g], state=state, weight_decay=0.1), ops.AdamW([ws], [gs], state=state, weight_decay=0.1)
+    large.step(1e-2)
+    small.step(1e-2)
+    assert torch.equal(w[n - tail:], ws)
+    if state == "f32":
+        assert torch.equal(large.m[n - tail:n], small.m[:tail]) and torch.equal(large.v[n - tail:n], small.v[:tail])
+    else:
+        m, u = large.unpack(torch.bfloat16)
+        m2, u2 = small.unpack(torch.bfloat16)
+        # either is within a whole step of what both round: 1/8 and 1/16 of the value, or of the block's smallest step
+        for a, b, share in ((m[n - tail:n].float(), m2[:tail].float(), 1 / 8), (u[n - tail:n].float(), u2[:tail].float(), 1 / 16)):
+            assert bool(((a - b).abs() <= 2 * share * torch.maximum(a.abs(), b.abs()) + float(b.abs().max()) * 2.0 ** -15).all())
+    large.step(1e-2, max_norm=1.0)
+    assert abs(float(large.grad_norm) - n ** 0.5) < 1e-3 * n ** 0.5

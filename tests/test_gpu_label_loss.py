@@ -549,3 +549,40 @@ def test_preference_of_long_sequences(env):
         ops.preference_loss(z, lab, torch.tensor(starts, device="cuda"), ref[:2].contiguous(), C, dlogits=room[10:M + 10])
         torch.cuda.synchronize()
         assert bool((room[:10] == 5).all()) and bool((room[M + 10:] == 5).all())
+
+
+@pytest.mark.parametrize("M,C,ldl", [(90_000_000, 21, 24), (33_000, 65_536, 65_600), (16_000, 140_000, 140_000)])
+def test_rows_behind_2_31_elements(env, M, C, ldl):
+    """Rows are worked on one by one: the last ones of a large call are, bit for bit, what a call on them alone gives."""
+    ops, torch = env
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of free memory")
+    _say("large", M, C)
+    assert M * ldl > 2 ** 31
+    z = torch.empty(M, ldl, dtype=torch.bfloat16, device="cuda").normal_()
+    lab = torch.randint(0, C, (M,), device="cuda")
+    n = 300
+    tail, tail_lab = z[M - n:].clone(), lab[M - n:].clone()
+    logp, lse = ops.label_logp(z, lab, C)
+    few, few_lse = ops.label_logp(tail, tail_lab, C)
+    assert torch.equal(logp[M - n:], few) and torch.equal(lse[M - n:], few_lse)
+    d = torch.empty_like(z)
+    up = torch.ones(M, device="cuda")
+    ops.label_logp_bwd(z, lab, lse, up, C, dlogits=d)
+    assert torch.equal(d[M - n:], ops.label_logp_bwd(tail, tail_lab, few_lse, up[:n].contiguous(), C))
+    old = logp - 0.1
+    sums, lp, _ = ops.policy_loss(z, lab, old, up, C, grad_scale=1.0, dlogits=d)
+    _, few_lp, few_d = ops.policy_loss(tail, tail_lab, old[M - n:].clone(), up[:n].contiguous(), C, grad_scale=1.0)
+    assert torch.equal(lp[M - n:], few_lp) and torch.equal(d[M - n:], few_d)
+    assert abs(float(sums[0]) / M + np.exp(0.1)) < 1e-5 and float(sums[3]) == 0
+    at = torch.tensor([0, M - n, M], device="cuda")
+    ref = torch.zeros(2, device="cuda")
+    _, seq, _ = ops.preference_loss(z, lab, at, ref, C, beta=1e-9, grad_scale=1e9, dlogits=d)
+    assert abs(float(seq[1]) - float(few.double().sum())) < 1e-6 * abs(float(seq[1]))
+    x = tail[:, :C].double()
+    lse64 = torch.logsumexp(x, 1)
+    ok = torch.ones(n, dtype=torch.bool, device="cuda")
+    h = 1e-9 * (float(seq[0]) - float(seq[1]))
+    coef = torch.full((n,), 1.0 / (1.0 + np.exp(h)), dtype=torch.float64, device="cuda")
+    tol = _reference(torch, tail, tail_lab, C)[4]
+    _check_grad(torch, d[M - n:], x, lse64, ok, tail_lab, coef, coef.abs() * 1e-6, tol, C)
