@@ -27,10 +27,10 @@ def short(name):
     return m.group(1) if m else name[:50]
 
 
-shutil.copy(newest(SRC + "/trace/runc/*_kernel_stats.csv"), "%s/%s_bench_kernel_stats.csv" % (DST, R))
+shutil.copy(newest(SRC + "/trace/*/*_kernel_stats.csv"), "%s/%s_bench_kernel_stats.csv" % (DST, R))
 shutil.copy(SRC + "/bench_line.json", "%s/%s_bench_line.json" % (DST, R))
 with open("%s/%s_bench_per_layer.txt" % (DST, R), "w") as f:
-    f.write(subprocess.check_output([sys.executable, "scripts/trace_layers.py", newest(SRC + "/trace/runc/*_kernel_trace.csv")]).decode())
+    f.write(subprocess.check_output([sys.executable, "scripts/trace_layers.py", newest(SRC + "/trace/*/*_kernel_trace.csv")]).decode())
 if os.path.exists(SRC + "/estep_bench.txt"):
     shutil.copy(SRC + "/estep_bench.txt", "%s/%s_estep_bench.txt" % (DST, R))
 
@@ -49,7 +49,7 @@ out = ["# rocprofv3 --pmc passes over `bench.py --steps 1 --warmup 1` (kernel-tr
        "# gfx950 correction (MI355X_MICROARCH.md, HBM): FETCH_SIZE under-reports wide coalesced reads by 2x -> hbm_read = 2*FETCH_SIZE*1024.", ""]
 agg = collections.OrderedDict()
 for sub in ("pmc_sq", "pmc_fetch", "pmc_write"):
-    rows = load(newest("%s/%s/runc/*_counter_collection.csv" % (SRC, sub)))
+    rows = load(newest("%s/%s/*/*_counter_collection.csv" % (SRC, sub)))
     conv = [r for r in rows if re.search(r"igemm|wgrad|conv_d64|conv_d4|conv_k32", r["name"])]
     conv = conv[len(conv) // 2:]  # second (timed) step
     for r in conv:
@@ -84,7 +84,7 @@ eout = ["# E-step kernels in the same rocprofv3 --pmc passes (last step): HBM-si
         "# gfx950 correction as above), L2 hit rate, wave-cycle split; algorithmic bytes (SURVEY 8d) = logits once + int64 labels.", ""]
 eagg = collections.OrderedDict()
 for sub in ("pmc_sq", "pmc_fetch", "pmc_write"):
-    rows = load(newest("%s/%s/runc/*_counter_collection.csv" % (SRC, sub)))
+    rows = load(newest("%s/%s/*/*_counter_collection.csv" % (SRC, sub)))
     es = [r for r in rows if re.search(r"estep", r["name"])]
     per_step = max(len(es) // 2, 1)
     for r in es[len(es) - per_step:]:
@@ -135,7 +135,7 @@ def full_rows(path):
 traffic = {c: {"read_bytes": 0.0, "write_bytes": 0.0, "launches": 0} for c in ("igemm_fwd", "igemm_dgrad", "igemm_wgrad")}
 per_kernel = collections.OrderedDict()
 for sub, counter, key, mult in (("pmc_fetch", "FETCH_SIZE", "read_bytes", 2 * 1024.0), ("pmc_write", "WRITE_SIZE", "write_bytes", 1024.0)):
-    rows = [r for r in full_rows(newest("%s/%s/runc/*_counter_collection.csv" % (SRC, sub))) if conv_kernel(r["full"]) is not None]
+    rows = [r for r in full_rows(newest("%s/%s/*/*_counter_collection.csv" % (SRC, sub))) if conv_kernel(r["full"]) is not None]
     assert len(rows) % 2 == 0, "expected two identical steps (--warmup 1 --steps 1)"
     conv = rows[len(rows) // 2:]   # the second (timed) step
     for r, c in zip(conv, classes_by_order([r["full"] for r in conv])):
