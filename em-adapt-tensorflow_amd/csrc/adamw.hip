@@ -85,8 +85,11 @@ struct AdamwScalars {
     float grad_scale;
     int clip, ignore_status;
 };
-// What is the same for all elements of a step, by one thread: whether it happens, the clip's factor, the bias corrections.
+// What is the same for all elements of a step, by one wave: whether it happens, the clip's factor, the bias corrections (a power to a lane).
 __device__ void adamw_control(AdamwControl *ctl, const AdamwScalars &a, double sum, unsigned *status) {
+    const long long t = ctl->steps + 1;
+    const double bias = 1.0 - pow(threadIdx.x & 1 ? a.beta2 : a.beta1, (double)t), bias1 = __shfl(bias, 0), bias2 = __shfl(bias, 1);
+    if (threadIdx.x != 0) return;
     bool go = a.ignore_status || !status_raised(status);
     float coef = a.grad_scale;
     if (a.clip) {
@@ -99,11 +102,10 @@ __device__ void adamw_control(AdamwControl *ctl, const AdamwScalars &a, double s
     }
     ctl->go = go ? 1u : 0u;
     if (!go) return;
-    const long long t = ctl->steps + 1;
     ctl->steps = t;
     ctl->coef = coef;
-    ctl->rate = (float)(a.lr / (1.0 - pow(a.beta1, (double)t)));
-    ctl->root2 = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)t)));
+    ctl->rate = (float)(a.lr / bias1);
+    ctl->root2 = (float)(1.0 / sqrt(bias2));
 }
 __global__ void adamw_control_kernel(AdamwControl *ctl, AdamwScalars a, unsigned *__restrict__ status) { adamw_control(ctl, a, 0.0, status); }
 
@@ -152,7 +154,7 @@ __global__ void __launch_bounds__(256) adamw_norm_kernel(const AdamwChunk *__res
     s = 0.0;
     for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) s += __hip_atomic_load(&ctl->sum[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     s = block_sum_f64(s, sh);
-    if (threadIdx.x != 0) return;
+    if (threadIdx.x >= 64) return;
     adamw_control(ctl, a, s, status);
 }
 
@@ -473,7 +475,7 @@ int emadapt_adamw_step(const void *table, int64_t chunks, int grad_dtype, int st
         if (bf) hipLaunchKernelGGL(adamw_norm_kernel<__bf16>, parts, dim3(256), 0, stream, tab, (long long)chunks, ctl, sc, status);
         else hipLaunchKernelGGL(adamw_norm_kernel<float>, parts, dim3(256), 0, stream, tab, (long long)chunks, ctl, sc, status);
     } else
-        hipLaunchKernelGGL(adamw_control_kernel, dim3(1), dim3(1), 0, stream, ctl, sc, status);
+        hipLaunchKernelGGL(adamw_control_kernel, dim3(1), dim3(64), 0, stream, ctl, sc, status);
     if (int rc = launch_status()) return rc;
     if (!chunks) return EMADAPT_OK;
     const AdamwArgs a = {(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, lr, seed, zero_grads};

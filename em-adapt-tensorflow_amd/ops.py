@@ -858,17 +858,19 @@ def _rows(logits, labels, num_classes, name="labels"):
         raise ValueError("logits must be [..., classes]")
     if labels.shape != shape[:-1]:
         raise ValueError("%s has shape %s, the logits' rows %s" % (name, tuple(labels.shape), tuple(shape[:-1])))
-    C = int(num_classes)
-    if not 0 < C <= shape[-1]:
-        raise ValueError("num_classes %d does not fit logits of %d columns" % (C, shape[-1]))
+    C, ldl = int(num_classes), shape[-1]
+    if not 0 < C <= ldl:
+        raise ValueError("num_classes %d does not fit logits of %d columns" % (C, ldl))
     _same_device(logits, labels, name)
-    return dt, shape[-1], labels.numel(), C
+    return dt, ldl, labels.numel(), C
 
 
 def _row_vector(t, logits, M, name):
     """Address of an f32 value per row (or None)."""
     if t is None:
         return None
+    if t.dtype is torch.float32 and t.numel() == M and t.is_contiguous() and t.get_device() == logits.get_device():
+        return t.data_ptr()
     _check(t, name=name)
     if t.numel() != M:
         raise ValueError("%s holds %d values, the logits %d rows" % (name, t.numel(), M))
@@ -886,8 +888,8 @@ def _dlogits(logits, dt, dlogits):
     return dlogits, ddt
 
 
-def _f32(shape, like):
-    return torch.empty(shape, dtype=torch.float32, device=like.device)
+def _f32(like, *shape):
+    return torch.empty(shape, dtype=torch.float32, device=like.device) if not shape else torch.empty(*shape, dtype=torch.float32, device=like.device)
 
 
 def _scratch(nbytes, like):
@@ -910,7 +912,7 @@ def label_logp(logits, labels, num_classes):
     """(logp f32 [...], lse f32 [...]): log-probability of the given labels and the rows' log-sum-exp.  logits f32 / bf16 [..., ldl], labels
     int64 [...]; a label outside [0, num_classes) has logp 0."""
     dt, ldl, M, C = _rows(logits, labels, num_classes)
-    logp = _f32(labels.shape, logits)
+    logp = _f32(logits, *labels.shape)
     lse = torch.empty_like(logp)
     _launch(logits, "emadapt_label_logp", logits.data_ptr(), dt, ldl, labels.data_ptr(), M, C, logp.data_ptr(), lse.data_ptr())
     return logp, lse
@@ -949,7 +951,7 @@ def policy_loss(logits, actions, old_logp, advantages, num_classes, ref_logp=Non
     ddt = DT_F32
     if want_grad:
         dlogits, ddt = _dlogits(logits, dt, dlogits)
-    sums, logp = _f32(4, logits), torch.empty_like(old_logp) if old_logp.shape == actions.shape else _f32(actions.shape, logits)
+    sums, logp = _f32(logits, 4), torch.empty_like(old_logp) if old_logp.shape == actions.shape else _f32(logits, *actions.shape)
     nbytes = _lib.load().emadapt_policy_loss_workspace_bytes(M, C)
     ws = _scratch(nbytes, logits)
     _launch(logits, "emadapt_policy_loss", logits.data_ptr(), dt, ldl, actions.data_ptr(), old, ref, adv, weight, M, C, clip_low, clip_high, kl_coef,
@@ -982,7 +984,7 @@ def preference_loss(logits, labels, seq_start, ref_logp, num_classes, beta=0.1, 
     ddt = DT_F32
     if want_grad:
         dlogits, ddt = _dlogits(logits, dt, dlogits)
-    loss, seq_logp = _f32(pairs, logits), _f32(2 * pairs, logits)
+    loss, seq_logp = _f32(logits, pairs), torch.empty_like(ref_logp) if ref_logp.dim() == 1 else _f32(logits, 2 * pairs)
     nbytes = _lib.load().emadapt_preference_loss_workspace_bytes(M, C)
     ws = _scratch(nbytes, logits)
     _launch(logits, "emadapt_preference_loss", logits.data_ptr(), dt, ldl, labels.data_ptr(), seq_start.data_ptr(), pairs, ref_logp.data_ptr(), M, C, beta,
