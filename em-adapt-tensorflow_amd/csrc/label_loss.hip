@@ -303,6 +303,7 @@ struct Outputs {
     unsigned char *near;        // rows to be looked at in 64 bits from their maximum in base (policy_finish_kernel)
     unsigned *ticket;           // its ticket, to be zeroed
     MaxSum *parts;              // [M][gridDim.y] of rows in several parts
+    float *sums;                // of a grid of one workgroup
 };
 
 // A row's part of the policy loss once its log-sum-exp is known, as f32 sees it; near: exact arithmetic may cut the ratio where f32 does not.
@@ -425,7 +426,9 @@ __global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs ou
         const double sum[4] = {t.loss, t.surrogate, t.kl, t.clipped};
         for (int k = 0; k < 4; k++) {
             const double v = block_sum_f64(sum[k], sh);
-            if (threadIdx.x == 0) out.partial[(long long)blockIdx.x * 4 + k] = v;
+            if (threadIdx.x != 0) continue;
+            if (out.sums) out.sums[k] = (float)v;
+            else out.partial[(long long)blockIdx.x * 4 + k] = v;
         }
     }
 }
@@ -867,13 +870,15 @@ Rows rows_of(const void *logits, int64_t ldl, const int64_t *labels, int64_t M, 
 //   loss alone  16 vectors, behind them statistics and rows' terms in two launches (f32 rows of 24: 52 us against 75 for 1.6 M, of 64: 106 against
 //               121, of 130: 135 against 114)
 template <int MODE, typename T, typename TD>
-bool launch_short(const Rows &a, const Policy &p, const Outputs &out, int cap, int *blocks, hipStream_t stream) {
+bool launch_short(const Rows &a, const Policy &p, Outputs out, int cap, int *blocks, hipStream_t stream) {
     const int64_t nvec = ceil_div(a.ldl, Vec<T>::N);
     if (nvec > (MODE == kLogp ? (a.last ? 384 : 512) : MODE == kPolicyGrad ? 384 : 16)) return false;
     int L = 1;
     while (L * 4 < nvec && L < 64) L *= 2;
     const bool three = nvec <= 3 * L;
     *blocks = (int)grid_of(ceil_div(a.M, 256 / L), cap);
+    if (MODE != kLogp && L <= kInlineLanes && a.M <= 1024 / L) *blocks = 1;   // (its sums are the whole ones, a launch less: 500 rows of 24 f32 16.6 us and 13.3)
+    if (*blocks > 1 || L > kInlineLanes) out.sums = nullptr;
 #define EMADAPT_GROUP(L, NV) hipLaunchKernelGGL((group_kernel<T, TD, L, NV, MODE>), dim3(*blocks), dim3(256), 0, stream, a, p, out)
     switch (L) {
         case 1: if (three) EMADAPT_GROUP(1, 3); else EMADAPT_GROUP(1, 4); break;
@@ -1003,7 +1008,7 @@ int launch_few(const Rows &a, const Policy &p, const MaxSum *parts, float *logp,
 template <typename T, typename TD>
 int policy_t(Rows a, Policy p, float *sums, float *logp, void *dlogits, int ddt, void *workspace, hipStream_t stream) {
     const PolicySpace w = policy_space(workspace, a.M);
-    Outputs out = {logp, nullptr, nullptr, nullptr, nullptr, dlogits, w.partial, nullptr, w.ticket, nullptr};
+    Outputs out = {logp, nullptr, nullptr, nullptr, nullptr, dlogits, w.partial, nullptr, w.ticket, nullptr, sums};
     int blocks = 0;
     unsigned finish = 1;
     if (a.M) {
@@ -1019,7 +1024,9 @@ int policy_t(Rows a, Policy p, float *sums, float *logp, void *dlogits, int ddt,
             done = launch_short<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
             if (!done && !few) done = launch_block<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
         }
-        if (done && ceil_div(a.ldl, Vec<T>::N) > kInlineLanes * 4) finish = grid_of(ceil_div(a.M, kFinishRows), kFinishBlocks);
+        const bool in_place = done && ceil_div(a.ldl, Vec<T>::N) <= kInlineLanes * 4;
+        if (in_place && blocks == 1) return launch_status();
+        if (done && !in_place) finish = grid_of(ceil_div(a.M, kFinishRows), kFinishBlocks);
         else out.near = nullptr;
         if (int rc = launch_status()) return rc;
         if (!done) {   // rows that no workgroup's registers hold, that are only read, or too few: log-sum-exp, the rows' terms, the gradient
