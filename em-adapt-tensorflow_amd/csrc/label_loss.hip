@@ -241,23 +241,59 @@ __device__ __forceinline__ float exp_minus_1(float q) {
     const float series = q * (1.f + q * (1.f / 2 + q * (1.f / 6 + q * (1.f / 24 + q * (1.f / 120 + q * (1.f / 720 + q * (1.f / 5040 + q * (1.f / 40320))))))));
     return fabsf(q) < 0.5f ? series : __expf(q) - 1.f;
 }
-// d loss / d logp of one row, and (count) what it adds to the sums.
-__device__ __forceinline__ float policy_row(float log_ratio, float q, bool has_ref, float adv, float w, const Policy &p, bool clipped, bool count,
-                                            PolicyTerms &t) {
-    const float free = -adv * __expf(log_ratio);
+// What one row adds to the sums before its weight, and its d loss / d logp.
+template <typename F> struct PolicyRow {
+    F loss, part, k, c;
+};
+__device__ __forceinline__ void policy_add(PolicyTerms &t, double w, double loss, double part, double k, bool clipped) {
+    t.loss += w * loss;
+    t.surrogate += w * part;
+    t.kl += w * k;
+    t.clipped += clipped ? w : 0.0;
+}
+// in f32, as far as its intermediates go (fits)
+__device__ __forceinline__ PolicyRow<float> policy_row(float log_ratio, float q, bool has_ref, float adv, float w, const Policy &p, bool clipped) {
+    const float free = adv == 0.f ? 0.f : -adv * __expf(log_ratio);   // (without an advantage nothing, whatever the ratio)
     const float e = has_ref ? exp_minus_1(q) : 0.f;
-    if (count) {
-        const float part = clipped ? -adv * (float)(adv > 0.f ? p.high : p.low) : free;
-        // exp(q) - 1 - q: from q^2 / 2 on where the rest cancels
-        const float k = !has_ref ? 0.f
-                        : fabsf(q) < 0.5f ? q * q * (1.f / 2 + q * (1.f / 6 + q * (1.f / 24 + q * (1.f / 120 + q * (1.f / 720 + q * (1.f / 5040 + q * (1.f / 40320)))))))
-                                          : e - q;
-        t.loss += (double)w * (double)(p.kl != 0.f ? part + p.kl * k : part);
-        t.surrogate += (double)w * (double)part;
-        t.kl += (double)w * (double)k;
-        t.clipped += clipped ? (double)w : 0.0;
-    }
-    return w * p.scale * ((clipped ? 0.f : free) - (p.kl != 0.f ? p.kl * e : 0.f));   // (e may have overflowed: no term, not 0 * inf)
+    PolicyRow<float> r;
+    r.part = clipped ? -adv * (float)(adv > 0.f ? p.high : p.low) : free;
+    // exp(q) - 1 - q: from q^2 / 2 on where the rest cancels
+    r.k = !has_ref ? 0.f
+          : fabsf(q) < 0.5f ? q * q * (1.f / 2 + q * (1.f / 6 + q * (1.f / 24 + q * (1.f / 120 + q * (1.f / 720 + q * (1.f / 5040 + q * (1.f / 40320)))))))
+                            : e - q;
+    r.loss = p.kl != 0.f ? r.part + p.kl * r.k : r.part;
+    r.c = w * p.scale * ((clipped ? 0.f : free) - (p.kl != 0.f ? p.kl * e : 0.f));   // (e may have overflowed: no term, not 0 * inf)
+    return r;
+}
+__device__ __forceinline__ bool fits(const PolicyRow<float> &r) { return fabsf(r.loss) < INFINITY && fabsf(r.c) < INFINITY; }
+// exp(x) where f32 may not hold it, as the eighth power of an f32 exponential.  Held at e^600: beyond what f32 factors bring back, and still finite, so
+// that a factor of 0 gives 0.
+__device__ __forceinline__ double wide_exp(float x) {
+    if (!(x > 80.f)) return (double)__expf(x);   // (NaN too)
+    double e = (double)__expf((x < 600.f ? x : 600.f) * 0.125f);
+    e *= e;
+    e *= e;
+    return e * e;
+}
+// exp(q) - 1 - q beyond f32 (q may be infinite)
+__device__ __forceinline__ double wide_k(float q) { return wide_exp(q) - 1.0 - (double)(q < 600.f ? q : 600.f); }
+// in 64 bits, of every row that is looked at again: an exponential beyond f32 (of an action that the old policy held for impossible, of a reference far
+// away) counts as what its factors make of it.  A coefficient that f32 cannot hold is held to its largest finite value: an infinite one gives NaN at
+// every class whose probability underflows.
+__device__ __forceinline__ PolicyRow<double> policy_row_wide(float log_ratio, float q, bool has_ref, double adv, double w, const Policy &p, bool clipped) {
+    const double free = -adv * wide_exp(log_ratio);
+    const bool small = fabsf(q) < 0.5f;
+    const double e = !has_ref ? 0.0 : small ? (double)exp_minus_1(q) : wide_exp(q) - 1.0;
+    PolicyRow<double> r;
+    r.part = clipped ? -adv * (adv > 0.0 ? p.high : p.low) : free;
+    r.k = !has_ref ? 0.0
+          : small ? (double)(q * q * (1.f / 2 + q * (1.f / 6 + q * (1.f / 24 + q * (1.f / 120 + q * (1.f / 720 + q * (1.f / 5040 + q * (1.f / 40320))))))))
+                  : wide_k(q);
+    r.loss = p.kl != 0.f ? r.part + (double)p.kl * r.k : r.part;
+    constexpr double kMost = 0x1.fffffep127;
+    const double c = w * (double)p.scale * ((clipped ? 0.0 : free) - (p.kl != 0.f ? (double)p.kl * e : 0.0));
+    r.c = c > kMost ? kMost : c < -kMost ? -kMost : c;   // (NaN stays)
+    return r;
 }
 // is the log of the ratio past the border that its advantage's sign puts up?
 __device__ __forceinline__ bool past_border(double log_ratio, float adv, const Policy &p) {
@@ -300,13 +336,14 @@ struct Outputs {
     float *base, *sum, *zero;   // kLogp: the rows' maximum and sum of exponentials; a value per row set to 0 (kPolicyGrad: base of the near rows)
     void *dlogits;
     double *partial;            // a workgroup's sums, [gridDim.x][4]
-    unsigned char *near;        // rows to be looked at in 64 bits from their maximum in base (policy_finish_kernel)
+    unsigned char *near;        // rows to be looked at again in 64 bits from their maximum in base (policy_finish_kernel)
     unsigned *ticket;           // its ticket, to be zeroed
     MaxSum *parts;              // [M][gridDim.y] of rows in several parts
     float *sums;                // of a grid of one workgroup
 };
 
-// A row's part of the policy loss once its log-sum-exp is known, as f32 sees it; near: exact arithmetic may cut the ratio where f32 does not.
+// A row's part of the policy loss once its log-sum-exp is known, as f32 sees it; near: to be looked at in 64 bits, since exact arithmetic may cut the ratio
+// where f32 does not, or since f32 does not hold the row's terms.
 struct PolicyInputs {
     float oldp, adv, w, refp;
     bool has_ref;
@@ -315,15 +352,22 @@ __device__ __forceinline__ PolicyInputs policy_inputs(const Policy &p, long long
     return {p.old_logp[r], p.adv[r], p.weight ? p.weight[r] : 1.f, p.ref_logp ? p.ref_logp[r] : 0.f, p.ref_logp != nullptr};
 }
 __device__ __forceinline__ float policy_of_row(const Policy &p, const PolicyInputs &x, float z, MaxSum row, bool count, float &lp, bool &near, PolicyTerms &t) {
-    const double lp64 = logp_of(z, row), lr = lp64 - (double)x.oldp;
+    const double lp64 = logp_of(z, row), lr = lp64 - (double)x.oldp, q = (double)x.refp - lp64;
     lp = (float)lp64;
+    const bool clipped = past_border(lr, x.adv, p);
+    const PolicyRow<float> r = policy_row((float)lr, (float)q, x.has_ref, x.adv, x.w, p, clipped);
     near = near_border(lr, x.adv, p);
-    return policy_row((float)lr, (float)((double)x.refp - lp64), x.has_ref, x.adv, x.w, p, past_border(lr, x.adv, p), count && !near, t);
+    if (!fits(r)) near |= lr == lr && q == q && x.adv == x.adv && x.w == x.w;   // (what is NaN stays so)
+    if (count && !near) policy_add(t, (double)x.w, (double)r.loss, (double)r.part, r.k < INFINITY ? (double)r.k : wide_k((float)q), clipped);   // (a KL part without a coefficient)
+    return r.c;
 }
 __device__ __forceinline__ float policy_of_exact(const Policy &p, const PolicyInputs &x, double lp64, bool count, float &lp, PolicyTerms &t) {
     const double lr = lp64 - (double)x.oldp;
     lp = (float)lp64;
-    return policy_row((float)lr, (float)((double)x.refp - lp64), x.has_ref, x.adv, x.w, p, past_border(lr, x.adv, p), count, t);
+    const bool clipped = past_border(lr, x.adv, p);
+    const PolicyRow<double> r = policy_row_wide((float)lr, (float)((double)x.refp - lp64), x.has_ref, (double)x.adv, (double)x.w, p, clipped);
+    if (count) policy_add(t, (double)x.w, r.loss, r.part, r.k, clipped);
+    return (float)r.c;
 }
 
 constexpr int kInlineLanes = 16;
@@ -331,10 +375,11 @@ constexpr int kInlineLanes = 16;
 // a wave's instruction (1.6 M rows of 24 f32: 54 us with a vector to a lane, 39 with three).  One pass: logits in, and with the policy loss their
 // gradient out; HBM bounds it from some 100000 rows on (logp of those rows 28.6 us in the kernel, 5.8 TB/s; 195312 rows of 1024 f32 65 us, 6.1),
 // below that the launches.  Policy: 64-bit logarithms and differences to each row keep narrow rows at 3 to 4 TB/s.
+// The bound: 4 waves to a SIMD, where the rows' 64-bit path would take the registers of one (40 M bf16 in rows of 128: 53.1 us with the bound, 58.7 without).
 template <typename T, typename TD, int L, int NV, int MODE>
-__global__ void __launch_bounds__(256) group_kernel(Rows a, Policy p, Outputs out) {
+__global__ void __launch_bounds__(256, MODE == kPolicyGrad ? 4 : 1) group_kernel(Rows a, Policy p, Outputs out) {
     constexpr int N = Vec<T>::N;
-    // Rows near a border here, or in policy_finish_kernel: 64-bit exponentials here double the registers of all rows (200 M bf16 in rows of 1000: 252 us
+    // Rows to be looked at again (near) here, or in policy_finish_kernel: 64-bit exponentials here double the registers of all rows (200 M bf16 in rows of 1000: 252 us
     // and 198), but find the row's inputs at hand (26896 rows of 24 f32, two of them near a border: 10.8 us and 20.5)
     constexpr bool kInline = L <= kInlineLanes;
     __shared__ double sh[4];

@@ -568,8 +568,10 @@ int emadapt_label_logp_bwd(const void *logits, int dtype, int64_t ldl, const int
  *   sums[4] = sum w (surrogate + kl_coef kl), sum w surrogate, sum w kl, sum w [the clip holds]
  *   dlogits = grad_scale * d sums[0] / d logits
  * weights f32 [M] or NULL (all 1); weight 0 takes the row out like a label outside [0, C).  Whether the clip holds is decided as
- * exact arithmetic on the inputs decides it (rows within rounding of a border are looked at in 64 bits).  clip_low in [0, 1],
- * clip_high >= 0.  logp f32 [M] is an output; dlogits may be NULL (the sums and logp alone). */
+ * exact arithmetic on the inputs decides it (rows within rounding of a border are looked at in 64 bits).  A ratio or an exp(q) beyond f32
+ * counts as what its factors make of it (nothing where the advantage is 0); a row's coefficient d (grad_scale sums[0]) / d logp that f32 does
+ * not hold is held to f32's largest finite value.  clip_low in [0, 1], clip_high >= 0.  logp f32 [M] is an output; dlogits may be NULL
+ * (the sums and logp alone). */
 size_t emadapt_policy_loss_workspace_bytes(int64_t M, int64_t C);
 int emadapt_policy_loss(const void *logits, int dtype, int64_t ldl, const int64_t *actions, const float *old_logp, const float *ref_logp,
                         const float *advantages, const float *weights, int64_t M, int64_t C, double clip_low, double clip_high,
