@@ -413,7 +413,8 @@ def launch_workers(n, worker_cmd, timeout=None, env=None, out=None):
     """`python bench.py --gpus N` without a launcher: start N fresh worker processes (one rank per GPU), relay rank 0's
     stdout (the one JSON line), return 0 only if every worker did.  Runs BEFORE anything in this process touches the GPU:
     the parent imports neither torch nor the HIP library, so the children are ordinary fork+exec of a GPU-free process.
-    When a worker fails the others are ended (exact PIDs, SIGTERM then SIGKILL) and its exit code is returned.
+    When a worker fails the others are ended (exact PIDs, SIGTERM then SIGKILL) and its exit code is returned; they get two seconds
+    to end by themselves first, in which a peer that is still starting, or fails for the same reason, says what it has to say.
 
     worker_cmd -- argv of one worker; RANK / LOCAL_RANK / WORLD_SIZE / LOCAL_WORLD_SIZE / MASTER_ADDR / MASTER_PORT are
                   supplied through the environment exactly as torch.distributed.run would.
@@ -480,6 +481,9 @@ def launch_workers(n, worker_cmd, timeout=None, env=None, out=None):
             "launcher received signal %d" % stop[0] if stop else "rank %d %s" % (
                 failed, "timed out" if rc == 124 else "exited with code %d" % rc), sum(procs[r].poll() is None for r in live)),
             file=sys.stderr)
+        grace = time.monotonic() + 2.0
+        while rc != 124 and not stop and time.monotonic() < grace and any(procs[r].poll() is None for r in live):
+            time.sleep(0.05)
         for r in live:
             if procs[r].poll() is None:
                 procs[r].send_signal(signal.SIGTERM)
