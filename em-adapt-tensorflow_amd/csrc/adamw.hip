@@ -43,9 +43,11 @@ constexpr int kRounds = 4, kChunk = 1024 * kRounds, kBlock = 64, kParts = 2048; 
 struct AdamwControl {
     long long steps;
     float norm, coef, rate, root2;   // of this step: the clip's factor and the bias corrections
-    unsigned go, ticket;             // whether it happens; the norm's workgroups that are done (0 between launches)
+    unsigned go, ticket;             // what happens (kNothing ..); the norm's workgroups that are done (0 between launches)
     double sum[kParts];
 };
+
+enum { kNothing = 0, kStep = 1, kClean = 2 };   // kClean: no update, but the gradients are zeroed where the step was asked to
 
 struct AdamwArgs {
     float b1, omb1, b2, omb2, eps;
@@ -90,18 +92,20 @@ __device__ void adamw_control(AdamwControl *ctl, const AdamwScalars &a, double s
     const long long t = ctl->steps + 1;
     const double bias = 1.0 - pow(threadIdx.x & 1 ? a.beta2 : a.beta1, (double)t), bias1 = __shfl(bias, 0), bias2 = __shfl(bias, 1);
     if (threadIdx.x != 0) return;
-    bool go = a.ignore_status || !status_raised(status);
+    unsigned go = a.ignore_status || !status_raised(status) ? kStep : kNothing;
     float coef = a.grad_scale;
     if (a.clip) {
         const double norm = fabs((double)a.grad_scale) * sqrt(sum);
         ctl->norm = (float)norm;
         if (!(norm <= 1.7976931348623157e308)) {
-            if (go) status_raise(status, EMADAPT_STATUS_NAN_GRADIENT);
-            go = false;
+            if (go) {   // (an accumulator would keep what is not finite for good)
+                status_raise(status, EMADAPT_STATUS_NAN_GRADIENT);
+                go = kClean;
+            }
         } else if (norm > a.max_norm) coef = (float)((double)a.grad_scale * (a.max_norm / norm));
     }
-    ctl->go = go ? 1u : 0u;
-    if (!go) return;
+    ctl->go = go;
+    if (go != kStep) return;
     ctl->steps = t;
     ctl->coef = coef;
     ctl->rate = (float)(a.lr / bias1);
@@ -186,14 +190,25 @@ __device__ __forceinline__ Element adamw_element(float g, float m, float v, floa
 }
 __device__ __forceinline__ bool finite(const Element &e) { return fabsf(e.m) < INFINITY && e.v < INFINITY; }
 
+// the clean op alone, on element i of a chunk and every `step`-th after it
+template <typename TG> __device__ __forceinline__ void zero_chunk(const AdamwChunk &c, int i, int step) {
+    EMADAPT_GLOBAL TG *g = global<TG>(c.g);
+    for (; i < c.n; i += step) g[i] = (TG)0.f;
+}
+
 // A workgroup to a chunk: of a whole one all 16 loads are in flight before the first is used.  (Fewer workgroups that walk several chunks each are
 // slower: 351 us with 2048 of them against 323 for 65.1 M parameters.)  Last chunks first: the norm has just read their gradients.  Everything
 // else is read and written once and told so (nontemporal), so that the gradients stay in the cache from the norm to here: 403 -> 329 us.
 template <typename TG>
 __global__ void __launch_bounds__(256) adamw_f32_kernel(const AdamwChunk *__restrict__ table, const AdamwControl *__restrict__ ctl, AdamwArgs a,
                                                        unsigned *__restrict__ status) {
-    if (!ctl->go) return;
+    const unsigned go = ctl->go;
+    if (!go) return;
     const AdamwChunk c = table[gridDim.x - 1 - blockIdx.x];
+    if (go == kClean) {
+        if (a.zero_grads) zero_chunk<TG>(c, threadIdx.x, 256);
+        return;
+    }
     const float rate = mul_rn(ctl->rate, c.ls), fade = (float)(a.lr * (double)c.ls * (double)c.wd), coef = ctl->coef, root2 = ctl->root2;
     EMADAPT_GLOBAL TG *gp = global<TG>(c.g);
     EMADAPT_GLOBAL float *wp = global<float>(c.w), *mp = global<float>(c.m), *vp = global<float>(c.v);
@@ -320,9 +335,13 @@ __device__ __forceinline__ bool adamw_codes(Codes &c, const float (&g)[4], float
 template <typename TG>
 __global__ void __launch_bounds__(256) adamw_u8_kernel(const AdamwChunk *__restrict__ table, const AdamwControl *__restrict__ ctl, AdamwArgs a,
                                                       unsigned *__restrict__ status) {
-    if (!ctl->go) return;
-    const unsigned at = gridDim.x - 1 - blockIdx.x;
+    const unsigned go = ctl->go, at = gridDim.x - 1 - blockIdx.x;
+    if (!go) return;
     const AdamwChunk c = table[at / kRounds];
+    if (go == kClean) {
+        if (a.zero_grads) zero_chunk<TG>(c, (int)(at % kRounds) * 256 + threadIdx.x, 256 * kRounds);
+        return;
+    }
     const int i = (int)(at % kRounds) * 256 + threadIdx.x, n4 = c.n - i * 4;   // (n4: the thread's elements, may be more than 4)
     if (n4 + (int)(threadIdx.x & 15) * 4 <= 0) return;                          // (whole rows of lanes: the codes' buffers reach that far)
     const float rate = mul_rn(ctl->rate, c.ls), fade = (float)(a.lr * (double)c.ls * (double)c.wd);

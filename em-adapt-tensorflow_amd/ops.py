@@ -1085,8 +1085,8 @@ class AdamW:
         self._grads_apart = None
 
     def step(self, lr, grad_scale=1.0, max_norm=0.0, zero_grads=False):
-        """One step on the current stream (steps of one object belong on one stream, or in order): gradients times grad_scale, held to the global norm max_norm (0: not), weights and moments updated in place.  zero_grads: the
-        gradients are zeroed behind it.  A gradient (or norm) that is not finite leaves its elements (or the whole step) out and raises
+        """One step on the current stream (steps of one object belong on one stream, or in order): gradients times grad_scale, held to the global norm
+        max_norm (0: not), weights and moments updated in place.  zero_grads: the gradients are zeroed behind it, also where their norm refuses it.  A gradient (or norm) that is not finite leaves its elements (or the whole step) out and raises
         STATUS_NAN_GRADIENT of the device status word; while the word is raised the step does nothing (status_poll).  A captured step replays with the
         lr, grad_scale and max_norm of its capture, and counts on."""
         if zero_grads and not self._grads_apart:

@@ -606,7 +606,8 @@ int emadapt_preference_loss(const void *logits, int dtype, int64_t ldl, const in
  * replayed; two steps on one control block belong on one stream.
  * A raised status word makes the step a no-op (not in collective mode: the gradient carries the failure).  A norm that is not finite
  * makes the step a no-op; an element whose moments would leave the finite numbers is left alone; both raise EMADAPT_STATUS_NAN_GRADIENT.
- * zero_grads: the gradients are zeroed behind the step (the clean op of deeplab.py:204).  beta1, beta2 in [0, 1), eps >= 1e-16; lr, grad_scale,
+ * zero_grads: the gradients are zeroed behind the step (the clean op of deeplab.py:204), also where their norm refuses it; not while the
+ * word was raised before.  beta1, beta2 in [0, 1), eps >= 1e-16; lr, grad_scale,
  * weight_decay and lr_scale finite. */
 #define EMADAPT_ADAMW_F32 0
 #define EMADAPT_ADAMW_U8 1
