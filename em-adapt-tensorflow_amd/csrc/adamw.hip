@@ -481,7 +481,7 @@ int emadapt_adamw_step(const void *table, int64_t chunks, int grad_dtype, int st
         !isfinite(lr) || !isfinite(grad_scale))
         return EMADAPT_ERR_INVALID;
     if (!control || control_bytes < sizeof(AdamwControl)) return EMADAPT_ERR_WORKSPACE;
-    if (chunks > 0x7FFFFFFF / kRounds) return EMADAPT_ERR_UNSUPPORTED;
+    if (chunks > 0x7FFFFFFF / kRounds) return EMADAPT_ERR_UNSUPPORTED;   // (2 T elements)
     hipStream_t stream = as_stream(stream_);
     const AdamwChunk *tab = static_cast<const AdamwChunk *>(table);
     AdamwControl *ctl = static_cast<AdamwControl *>(control);
@@ -498,16 +498,23 @@ int emadapt_adamw_step(const void *table, int64_t chunks, int grad_dtype, int st
     if (int rc = launch_status()) return rc;
     if (!chunks) return EMADAPT_OK;
     const AdamwArgs a = {(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, lr, seed, zero_grads};
-    const dim3 grid((unsigned)chunks), block(256);
-    if (state == EMADAPT_ADAMW_F32) {
-        if (bf) hipLaunchKernelGGL(adamw_f32_kernel<__bf16>, grid, block, 0, stream, tab, ctl, a, status);
-        else hipLaunchKernelGGL(adamw_f32_kernel<float>, grid, block, 0, stream, tab, ctl, a, status);
-    } else {
-        const dim3 rounds((unsigned)(chunks * kRounds));
-        if (bf) hipLaunchKernelGGL(adamw_u8_kernel<__bf16>, rounds, block, 0, stream, tab, ctl, a, status);
-        else hipLaunchKernelGGL(adamw_u8_kernel<float>, rounds, block, 0, stream, tab, ctl, a, status);
+    // (a grid has fewer than 2^32 threads: one launch up to 2^24 chunks, 2^22 in 8 bits; last chunks first, as in the kernels)
+    const int64_t rounds = state == EMADAPT_ADAMW_U8 ? kRounds : 1, most = 0xFFFFFFFFll / (256 * rounds);
+    for (int64_t left = chunks; left > 0;) {
+        const int64_t n = left < most ? left : most;
+        left -= n;
+        const dim3 grid((unsigned)(n * rounds)), block(256);
+        const AdamwChunk *from = tab + left;
+        if (state == EMADAPT_ADAMW_F32) {
+            if (bf) hipLaunchKernelGGL(adamw_f32_kernel<__bf16>, grid, block, 0, stream, from, ctl, a, status);
+            else hipLaunchKernelGGL(adamw_f32_kernel<float>, grid, block, 0, stream, from, ctl, a, status);
+        } else {
+            if (bf) hipLaunchKernelGGL(adamw_u8_kernel<__bf16>, grid, block, 0, stream, from, ctl, a, status);
+            else hipLaunchKernelGGL(adamw_u8_kernel<float>, grid, block, 0, stream, from, ctl, a, status);
+        }
+        if (int rc = launch_status()) return rc;
     }
-    return launch_status();
+    return EMADAPT_OK;
 }
 
 int emadapt_adamw_unpack(const void *m_codes, const void *u_codes, const void *powers, int64_t n, void *m, void *u, int dtype, void *stream_) {
