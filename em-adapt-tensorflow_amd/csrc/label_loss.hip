@@ -1171,8 +1171,17 @@ int emadapt_preference_loss(const void *logits, int dtype, int64_t ldl, const in
         if (parts > 1) {
             hipLaunchKernelGGL(preference_part_kernel, dim3((unsigned)parts, (unsigned)(2 * pairs)), dim3(1024), 0, stream, p);
             hipLaunchKernelGGL(preference_pair_kernel<true>, dim3((unsigned)parts, (unsigned)pairs), dim3(1024), 0, stream, p);
-        } else
-            hipLaunchKernelGGL(preference_pair_kernel<false>, dim3((unsigned)pairs), dim3(1024), 0, stream, p);
+        } else {
+            constexpr int64_t kMost = 0xFFFFFFFFll / 1024;   // (a grid has fewer than 2^32 threads)
+            for (int64_t at = 0; at < pairs; at += kMost) {
+                Preference some = p;
+                some.seq_start += 2 * at;
+                some.ref += 2 * at;
+                some.loss += at;
+                some.seq_logp += 2 * at;
+                hipLaunchKernelGGL(preference_pair_kernel<false>, dim3((unsigned)(pairs - at < kMost ? pairs - at : kMost)), dim3(1024), 0, stream, some);
+            }
+        }
         if (int rc = launch_status()) return rc;
     }
     if (M && dlogits) return launch_grad(a, dtype, base, sum, coef, dlogits, dlogits_dtype, stream);
