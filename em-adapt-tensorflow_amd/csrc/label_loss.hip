@@ -897,6 +897,8 @@ inline unsigned grid_of(int64_t n, int64_t cap) { return (unsigned)(n < 1 ? 1 : 
 int check_rows(const void *logits, int dtype, int64_t ldl, const int64_t *labels, int64_t M, int64_t C, const void *grad, int grad_dtype) {
     if (!is_dt(dtype) || (grad && !is_dt(grad_dtype)) || M < 0 || C <= 0 || ldl < C) return EMADAPT_ERR_INVALID;
     if (ldl > (int64_t)1 << 30 || M > ((int64_t)1 << 48) / ldl) return EMADAPT_ERR_UNSUPPORTED;
+    // (a grid has fewer than 2^32 threads, of which each writes the gradient of at most four vectors, in whole workgroups to each of a few rows)
+    if (grad && M * ceil_div(ldl, 16 / (int64_t)dt_size(dtype)) > ((int64_t)1 << 34) - (1 << 20)) return EMADAPT_ERR_UNSUPPORTED;
     if (M == 0) return EMADAPT_OK;
     if (!logits || !labels || !aligned(logits, dt_size(dtype)) || !aligned(labels, 8) || (grad && !aligned(grad, dt_size(grad_dtype)))) return EMADAPT_ERR_INVALID;
     // (the rows are read again after other rows' gradients are written)
@@ -986,8 +988,7 @@ int launch_grad_t(const Rows &a, const float *base, const float *sum, const floa
     const int64_t nvec = ceil_div(a.ldl, Vec<T>::N), total = nvec * a.M;
     // four vectors to a thread, or one where that leaves CUs without a workgroup (40344 rows of 24 f32: 7.7 us and 4.1)
     const bool four = total >= 4 * 256 * 1024;
-    const int64_t blocks = ceil_div(total, four ? 1024 : 256);
-    if (blocks > 0x7FFFFFFF) return EMADAPT_ERR_UNSUPPORTED;
+    const int64_t blocks = ceil_div(total, four ? 1024 : 256);   // (check_rows: not more threads than a grid has)
 #define EMADAPT_GRAD(TD, U, SUM) \
     hipLaunchKernelGGL((row_grad_kernel<T, TD, U, SUM>), dim3((unsigned)blocks), dim3(256), 0, stream, a, base, sum, coef, static_cast<TD *>(d), (unsigned)nvec, (long long)total)
 #define EMADAPT_GRAD_OF(SUM)                                             \
