@@ -298,7 +298,7 @@ class ADAPT(Network):
         self.net[layer] = None
 
     def _allocate_flat(self):
-        """One flat buffer each for params / grads / accumulators / momentum, fc8 first (backward order)."""
+        """One flat buffer each for params / grads / accumulators (and momentum, if that is the optimizer), fc8 first (backward order)."""
         order = list(self._shapes.keys())  # build order from the dry pass
         self._segments = {}
         off = 0
@@ -316,9 +316,10 @@ class ADAPT(Network):
             params=torch.zeros(total, dtype=torch.float32, device=dev),
             grads=torch.zeros(total, dtype=torch.float32, device=dev),
             accum=torch.zeros(total, dtype=torch.float32, device=dev),
-            momentum=torch.zeros(total, dtype=torch.float32, device=dev),
             total=total,
         )
+        if self.optimizer == "momentum":   # (AdamW keeps its own states, from optimize() on)
+            self._flat["momentum"] = torch.zeros(total, dtype=torch.float32, device=dev)
         for layer, seg in self._segments.items():
             s, nw, nb = seg["start"], seg["nw"], seg["nb"]
             kh, kw, cin, cout = seg["shape"]

@@ -180,7 +180,7 @@ class _Saver:
         for layer, (w, b) in n.weights.items():
             blob[layer + "_weights"] = w.detach().cpu().numpy()
             blob[layer + "_bias"] = b.detach().cpu().numpy()
-            if getattr(n, "_flat", None) is not None and getattr(n, "_adamw", None) is None:
+            if "momentum" in (getattr(n, "_flat", None) or {}):
                 vw, vb = self._momentum_views(layer)
                 blob[layer + "_weights/Momentum"] = vw.detach().cpu().numpy()
                 blob[layer + "_bias/Momentum"] = vb.detach().cpu().numpy()
@@ -223,7 +223,7 @@ class _Saver:
             for layer, (w, b) in n.weights.items():
                 w.copy_(torch.from_numpy(z[layer + "_weights"]).to(w.device))
                 b.copy_(torch.from_numpy(z[layer + "_bias"]).to(b.device))
-                if flat is not None and layer + "_weights/Momentum" in z.files:
+                if "momentum" in (flat or {}) and layer + "_weights/Momentum" in z.files:
                     vw, vb = self._momentum_views(layer)
                     vw.copy_(torch.from_numpy(z[layer + "_weights/Momentum"]).to(vw.device))
                     vb.copy_(torch.from_numpy(z[layer + "_bias/Momentum"]).to(vb.device))
@@ -239,7 +239,9 @@ class _Saver:
                     adamw.steps.copy_(torch.from_numpy(z["adam_steps"]).to(adamw.device))
                 else:
                     warnings.warn("checkpoint %s holds no %s moments of AdamW -- weights restored, the moments left as they are" % (path, adamw.state))
-            elif flat is not None and slots == 0:
+            elif "momentum" not in (flat or {}):
+                pass   # (no optimizer state here yet: weights alone)
+            elif slots == 0:
                 # round-1 files hold the whole (padded) momentum buffer as one array: usable when the layout still matches
                 if _LEGACY_MOMENTUM in z.files and z[_LEGACY_MOMENTUM].size == flat["momentum"].numel():
                     flat["momentum"].copy_(torch.from_numpy(z[_LEGACY_MOMENTUM]).reshape(-1).to(flat["momentum"].device))
@@ -248,7 +250,7 @@ class _Saver:
                            if _LEGACY_MOMENTUM in z.files else "it holds no momentum slots")
                     warnings.warn("checkpoint %s: %s -- weights restored, momentum left as it is (zero in a fresh run), "
                                   "as with the reference's weights-only Saver" % (path, why))
-            elif flat is not None and slots != len(n.weights):
+            elif slots != len(n.weights):
                 raise ValueError("checkpoint %s holds momentum slots for %d of %d layers" % (path, slots, len(n.weights)))
         if flat is not None:
             n._flat["params"].add_(0)   # bump torch's version counter: derived filter images are refreshed
