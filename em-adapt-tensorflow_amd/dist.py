@@ -12,7 +12,8 @@ below the completed watermark is all-reduced asynchronously (torch.distributed: 
 which runs the collective on its own HIP stream behind the compute stream's current position), so the
 fc8/fc7/fc6 gradients -- 77 % of the bytes -- travel while conv5..conv1 are still being differentiated.
 ``wait()`` joins the outstanding collectives before the optimiser step.  Works unchanged on CPU tensors
-with the gloo backend (tests).
+with the gloo backend (tests); GPU tensors in a gloo job (a rehearsal of several ranks on one GPU) are copied to the
+host and back around each collective.
 
 WHEN the collectives may start is the caller's decision.  The default is launch-on-completion: the exchange has nearly the
 whole backward pass (~55 ms in fp32) to hide in.  ``hold()`` / ``release()`` let a step keep completed buckets back until a
@@ -62,6 +63,15 @@ def _ops():
     return ops
 
 
+def _through_host(is_cuda, group=None):
+    """gloo is given CPU tensors only (its collectives on device tensors have hung where ranks share a GPU): GPU tensors travel through host copies."""
+    return is_cuda and dist.get_backend(group) == "gloo"
+
+
+def _host(t):
+    return t.detach().to("cpu", copy=True)   # (synchronous, on the current stream)
+
+
 class GradSync:
     def __init__(self, flat, segments, bucket_bytes=64 << 20, group=None, algo="allreduce", payload="fp32", writeback=True, prepacked=False,
                  boundaries=None):
@@ -87,6 +97,7 @@ class GradSync:
         self.prepacked = bool(prepacked) and algo == "direct" and not self.writeback
         self.sendfull = None
         self.gathered = None
+        self.through_host = _through_host(flat.is_cuda, group)
         self.world_size = dist.get_world_size(group)
         self.rank = dist.get_rank(group)
         self.total = max(e for _, e in segments)
@@ -170,7 +181,12 @@ class GradSync:
                 send[:n].copy_(self.flat[s:e])
                 if npad > n:
                     send[n:].zero_()
-        dist.all_to_all_single(recv, send, group=self.group)
+        if self.through_host:
+            there, back = _host(send), torch.empty(npad, dtype=recv.dtype)
+            dist.all_to_all_single(back, there, group=self.group)
+            recv.copy_(back)
+        else:
+            dist.all_to_all_single(recv, send, group=self.group)
         out = self._shard_p[:sh]
         if hip:
             _ops().grad_owner_sum(recv, W, out)      # ranks 0, 1, 2, ... added in fp32, rounded once: one pass
@@ -181,7 +197,12 @@ class GradSync:
                 acc.add_(recv[r * sh:(r + 1) * sh])
             if self.payload == "bf16":
                 out.copy_(acc)                       # the sum, rounded once
-        dist.all_gather_into_tensor(gath, out, group=self.group)
+        if self.through_host:
+            there, back = _host(out), torch.empty(npad, dtype=gath.dtype)
+            dist.all_gather_into_tensor(back, there, group=self.group)
+            gath.copy_(back)
+        else:
+            dist.all_gather_into_tensor(gath, out, group=self.group)
         if self.writeback:
             self.flat[s:e].copy_(gath[:n])
 
@@ -226,6 +247,10 @@ class GradSync:
                     self._side_used = True
                 else:
                     self._exchange_direct(s, e)
+            elif self.through_host:
+                there = _host(view)
+                dist.all_reduce(there, op=dist.ReduceOp.SUM, group=self.group)
+                view.copy_(there)
             else:
                 self._works.append(dist.all_reduce(view, op=dist.ReduceOp.SUM, group=self.group, async_op=True))
             self.launched_bytes += view.numel() * view.element_size()
@@ -279,6 +304,8 @@ class GradSync:
 
 def all_reduce_max(value, device):
     """MAX over ranks of a host float (bench timing)."""
+    if _through_host(torch.device(device).type == "cuda"):
+        device = "cpu"
     t = torch.tensor([float(value)], dtype=torch.float64, device=device)
     dist.all_reduce(t, op=dist.ReduceOp.MAX)
     return float(t.item())
