@@ -647,7 +647,7 @@ class ADAPT(Network):
         self.net["lr"] = float(base_lr)
         self._momentum = float(momentum)
         if self.optimizer != "momentum":
-            params, decay = [], []
+            before, params, decay = self._adamw, [], []
             for layer in self._segments:
                 s, nw, nb = (self._segments[layer][k] for k in ("start", "nw", "nb"))
                 params += [self._flat["params"][s:s + nw], self._flat["params"][s + nw:s + nw + nb]]
@@ -655,6 +655,10 @@ class ADAPT(Network):
             self._adamw = ops.AdamW(params, self._adamw_grads(self._flat["accum"]), state="u8" if self.optimizer == "adamw8" else "f32",
                                     betas=tuple(self.config.get("betas", (0.9, 0.999))), eps=float(self.config.get("adam_eps", 1e-8)),
                                     weight_decay=decay, seed=self.seed)
+            if before is not None:   # (trained before: the moments and steps go on, as the Momentum buffer does)
+                for name in ("m", "v") if before.state == "f32" else ("m8", "u8", "powers"):
+                    getattr(self._adamw, name).copy_(getattr(before, name))
+                self._adamw.steps.copy_(before.steps)
             self._adamw_source = self._flat["accum"]
         # the three "ops" of the reference's loop (deeplab.py:202-205), as callables
         self.net["accum_gradient"] = self._flat["accum"]
