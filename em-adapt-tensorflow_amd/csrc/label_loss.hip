@@ -374,13 +374,16 @@ constexpr int kInlineLanes = 16;
 // L lanes to a row, NV vectors of the padded row to a lane: few lanes, so that what is done once a row (logarithm, loss) is done for many rows by
 // a wave's instruction (1.6 M rows of 24 f32: 54 us with a vector to a lane, 39 with three).  One pass: logits in, and with the policy loss their
 // gradient out; HBM bounds it from some 100000 rows on (logp of those rows 28.6 us in the kernel, 5.8 TB/s; 195312 rows of 1024 f32 65 us, 6.1),
-// below that the launches.  Policy: 64-bit logarithms and differences to each row keep narrow rows at 3 to 4 TB/s.
+// below that the launches.  Narrow policy rows stay at 3 to 4 TB/s.  With the gradient its stores bound them, of which one covers 32 of every 96 bytes
+// (1.67 M rows of 24 f32: 118 us, 63 without the stores, 121 with them and without the loss's arithmetic), without it each row's arithmetic (58 us,
+// 35 without).
 // The bound: 4 waves to a SIMD, where the rows' 64-bit path would take the registers of one (40 M bf16 in rows of 128: 53.1 us with the bound, 58.7 without).
 template <typename T, typename TD, int L, int NV, int MODE>
 __global__ void __launch_bounds__(256, MODE == kPolicyGrad ? 4 : 1) group_kernel(Rows a, Policy p, Outputs out) {
     constexpr int N = Vec<T>::N;
-    // Rows to be looked at again (near) here, or in policy_finish_kernel: 64-bit exponentials here double the registers of all rows (200 M bf16 in rows of 1000: 252 us
-    // and 198), but find the row's inputs at hand (26896 rows of 24 f32, two of them near a border: 10.8 us and 20.5)
+    // Rows to be looked at again (near) here, or in policy_finish_kernel: 64-bit exponentials here double the registers of all rows (200 M bf16 in rows of 1000:
+    // 252 us and 198), but find the row's inputs at hand (26896 rows of 24 f32, two of them near a border: 10.8 us and 20.5; none of them: 9.7 and 12.5;
+    // 1.67 M rows: 118 and 137, of 24 bf16 46 and 58)
     constexpr bool kInline = L <= kInlineLanes;
     __shared__ double sh[4];
     const int lane = threadIdx.x % L;
@@ -496,10 +499,10 @@ template <int N> __device__ __forceinline__ void take(const float (&v)[N], float
     m = top;
 }
 
-// A workgroup of W waves to a row, NV whole vectors to a thread, and the C % N last elements one to a thread.  HBM bounds it, each logit read and
+// The policy loss with its gradient by a workgroup of W waves to a row, NV whole vectors to a thread, and the C % N last elements one to a thread.  HBM bounds it, each logit read and
 // each gradient written once: 4096 x 65536 bf16 199 us, 5.4 TB/s of the 4.8 to 5.3 that a copy of that size reaches (330 us where statistics and
 // gradient each read the logits).
-template <typename T, typename TD, int W, int NV, int MODE>
+template <typename T, typename TD, int W, int NV>
 __global__ void __launch_bounds__(64 * W, 4) block_kernel(Rows a, Policy p, Outputs out) {
     constexpr int N = Vec<T>::N, kThreads = 64 * W;
     __shared__ MaxSum pair[2][W];
@@ -657,7 +660,7 @@ __device__ void policy_rows(const Rows &a, const Policy &p, const MaxSum *__rest
             logp[r] = lp;
             if (!PARTS) coef[r] = f;
         }
-        // rows near a border, in the order of their index
+        // rows to be looked at again, in the order of their index
         const unsigned long long b = __ballot(again);
         if ((threadIdx.x & 63) == 0) mask[threadIdx.x >> 6] = b;
         __syncthreads();
@@ -693,7 +696,7 @@ __global__ void __launch_bounds__(256) policy_row_kernel(Rows a, Policy p, const
 }
 // Few long rows, whose statistics came in parts: the first workgroup writes logp and the sums, the others the gradient of 256 kUnroll vectors of
 // one row each (per: workgroups to a row), whose term each of them takes from the parts by itself -- a launch less than with the terms in one of
-// their own (7 rows of 128001 bf16: 20.9 us and 17.5, 128 rows: 35 and 26).  In a row near a border each of them goes through the row.
+// their own (7 rows of 128001 bf16: 20.9 us and 17.5, 128 rows: 35 and 26).  In a row to be looked at again each of them goes through it.
 template <typename T, typename TD, int kUnroll>
 __global__ void __launch_bounds__(256) policy_few_kernel(Rows a, Policy p, const MaxSum *__restrict__ parts, float *__restrict__ logp, float *__restrict__ sums,
                                                         TD *__restrict__ dlogits, unsigned per) {
@@ -734,7 +737,7 @@ __global__ void __launch_bounds__(256) policy_few_kernel(Rows a, Policy p, const
 }
 
 constexpr int kFinishRows = 16 * 1024;   // to a workgroup
-// The sums of the launch before, and its rows near a border (near, or null) in 64 bits: most workgroups find none.
+// The sums of the launch before, and its rows to be looked at again (near, of a launch that wrote a gradient; or null) in 64 bits: most workgroups find none.
 // Their terms were left out there; logp and the gradient are written again.  The last workgroup adds everything up in a fixed order.
 template <typename T, typename TD>
 __global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, Outputs out, int nparts, double *__restrict__ fixed, float *__restrict__ sums) {
@@ -769,7 +772,6 @@ __global__ void __launch_bounds__(1024) policy_finish_kernel(Rows a, Policy p, O
                 float lp;
                 const float f = policy_of_exact(p, policy_inputs(p, r), lp64, first == 0, lp, t);
                 if (first == 0) out.logp[r] = lp;
-                if (!out.dlogits) return;
                 TD *d = static_cast<TD *>(out.dlogits) + r * a.ldl;
                 const float over = (float)((double)f / sum);
 #pragma unroll 1
@@ -946,13 +948,13 @@ bool launch_short(const Rows &a, const Policy &p, Outputs out, int cap, int *blo
     return true;
 }
 // Rows of up to 16384 vectors in the registers of a workgroup.
-template <int MODE, typename T, typename TD>
+template <typename T, typename TD>
 bool launch_block(const Rows &a, const Policy &p, const Outputs &out, int cap, int *blocks, hipStream_t stream) {
     const int64_t nvec = a.C / Vec<T>::N;
     if (nvec < 1 || nvec > 16384) return false;   // (a thread without a vector of its own loads the row's last whole one: there has to be one)
     *blocks = (int)grid_of(a.M, cap);
     const dim3 grid(*blocks);
-#define EMADAPT_BLOCK(W, NV) hipLaunchKernelGGL((block_kernel<T, TD, W, NV, MODE>), grid, dim3(64 * W), 0, stream, a, p, out)
+#define EMADAPT_BLOCK(W, NV) hipLaunchKernelGGL((block_kernel<T, TD, W, NV>), grid, dim3(64 * W), 0, stream, a, p, out)
     if (nvec <= 512) EMADAPT_BLOCK(1, 8);
     else if (nvec <= 1024) EMADAPT_BLOCK(1, 16);
     else if (nvec <= 2048) EMADAPT_BLOCK(2, 16);
@@ -1068,7 +1070,7 @@ int policy_t(Rows a, Policy p, float *sums, float *logp, void *dlogits, int ddt,
         if (!dlogits) done = launch_short<kPolicy, T, T>(a, p, out, kPolicyBlocks, &blocks, stream);
         else {
             done = launch_short<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
-            if (!done && !few) done = launch_block<kPolicyGrad, T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
+            if (!done && !few) done = launch_block<T, TD>(a, p, out, kPolicyBlocks, &blocks, stream);
         }
         const bool in_place = done && ceil_div(a.ldl, Vec<T>::N) <= kInlineLanes * 4;
         if (in_place && blocks == 1) return launch_status();
