@@ -253,7 +253,7 @@ __device__ __forceinline__ void policy_add(PolicyTerms &t, double w, double loss
 }
 // in f32, as far as its intermediates go (fits)
 __device__ __forceinline__ PolicyRow<float> policy_row(float log_ratio, float q, bool has_ref, float adv, float w, const Policy &p, bool clipped) {
-    const float free = adv == 0.f ? 0.f : -adv * __expf(log_ratio);   // (without an advantage nothing, whatever the ratio)
+    const float free = adv == 0.f && log_ratio == log_ratio ? 0.f : -adv * __expf(log_ratio);   // (without an advantage nothing, however large the ratio)
     const float e = has_ref ? exp_minus_1(q) : 0.f;
     PolicyRow<float> r;
     r.part = clipped ? -adv * (float)(adv > 0.f ? p.high : p.low) : free;

@@ -130,3 +130,22 @@ def test_a_coefficient_beyond_f32_is_held(env, shape):
     sums, lp, d = ops.policy_loss(z, lab, torch.zeros_like(logp), adv, C, ref_logp=torch.full_like(logp, -1.0), kl_coef=0.1, grad_scale=1.0)
     assert bool((lp == float("-inf")).all()) and float(sums[0]) == float("inf") and not bool(torch.isnan(sums).any())
     assert bool(torch.isfinite(d).all()) and bool((d[:, 1] == -big).all())
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_nan_is_not_taken_for_an_overflow(env, shape):
+    """A row of NaN logits that counts stays NaN, without an advantage too; the rows beside it do not see it."""
+    ops, torch = env
+    M, C, ldl = shape
+    z = _logits(torch, M, ldl, "float32", 25)
+    lab = _labels(torch, M, C, 25, outside=False)
+    logp = ops.label_logp(z, lab, C)[0]
+    z[1, C // 2] = float("nan")
+    adv = torch.zeros(M, device="cuda")
+    for value in (0.0, -1.0):
+        adv[1] = value
+        for ref in (None, logp):
+            sums, lp, d = ops.policy_loss(z, lab, logp, adv, C, ref_logp=ref, kl_coef=0.0 if ref is None else 0.1, grad_scale=1.0)
+            assert bool(torch.isnan(lp[1])) and bool(torch.isnan(sums[:2]).all()) and bool(torch.isnan(d[1, :C]).all())
+            rest = torch.arange(M, device="cuda") != 1
+            assert bool(torch.isfinite(lp[rest]).all()) and bool(torch.isfinite(d[rest]).all())
