@@ -936,7 +936,7 @@ def policy_loss(logits, actions, old_logp, advantages, num_classes, ref_logp=Non
 
     old_logp, advantages, ref_logp, weights: f32 [...] (the last two optional).  Returns (sums f32 [4], logp f32 [...], dlogits or None); sums =
     weighted sums over the rows of the loss, its surrogate part, its KL part, and the rows whose ratio the clip holds; dlogits = grad_scale (default
-    1 / rows) times the gradient of sums[0]."""
+    1 / rows) times the gradient of sums[0], a row's factor held to f32's range."""
     dt, ldl, M, C = _rows(logits, actions, num_classes, "actions")
     if old_logp is None or advantages is None:
         raise ValueError("old_logp and advantages are needed")
@@ -1047,8 +1047,9 @@ class AdamW:
         self.set_grads(grads)
 
     def set_grads(self, grads):
-        """The gradients that step() reads from now on, also in a replay of a step that was captured with gradients of this type.  (Their addresses are
-        copied to the device, behind all work that is queued there: not under graph capture.)"""
+        """The gradients that step() reads from now on, also in a replay of a step that was captured with gradients of this type.  Their addresses are
+        copied to the device, behind all work that is queued there: a wait for the device and a table built on the host, so not under graph capture, and
+        better once than for every step (gradients that stay where they are need no second call)."""
         grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError("%d gradients for %d tensors" % (len(grads), len(self.params)))
@@ -1086,9 +1087,10 @@ class AdamW:
 
     def step(self, lr, grad_scale=1.0, max_norm=0.0, zero_grads=False):
         """One step on the current stream (steps of one object belong on one stream, or in order): gradients times grad_scale, held to the global norm
-        max_norm (0: not), weights and moments updated in place.  zero_grads: the gradients are zeroed behind it, also where their norm refuses it.  A gradient (or norm) that is not finite leaves its elements (or the whole step) out and raises
-        STATUS_NAN_GRADIENT of the device status word; while the word is raised the step does nothing (status_poll).  A captured step replays with the
-        lr, grad_scale and max_norm of its capture, and counts on."""
+        max_norm (0: not), weights and moments updated in place.  zero_grads: the gradients are zeroed behind it, also where their norm refuses it.  A
+        gradient (or norm) that is not finite leaves its elements (or the whole step) out and raises STATUS_NAN_GRADIENT of the device status word; while
+        the word is raised the step does nothing (status_poll).  A captured step replays with the lr, grad_scale and max_norm of its capture, and counts
+        on."""
         if zero_grads and not self._grads_apart:
             _refuse_overlap(self.grads, "grads")
             self._grads_apart = True
