@@ -277,9 +277,13 @@ __device__ __forceinline__ double wide_exp(float x) {
 }
 // exp(q) - 1 - q beyond f32 (q may be infinite)
 __device__ __forceinline__ double wide_k(float q) { return wide_exp(q) - 1.0 - (double)(q < 600.f ? q : 600.f); }
+// A row's coefficient: what f32 cannot hold is held to its largest finite value.  (An infinite one gives NaN at every class whose probability underflows.)
+__device__ __forceinline__ double held_to_f32(double c) {
+    constexpr double kMost = 0x1.fffffep127;
+    return c > kMost ? kMost : c < -kMost ? -kMost : c;   // (NaN stays)
+}
 // in 64 bits, of every row that is looked at again: an exponential beyond f32 (of an action that the old policy held for impossible, of a reference far
-// away) counts as what its factors make of it.  A coefficient that f32 cannot hold is held to its largest finite value: an infinite one gives NaN at
-// every class whose probability underflows.
+// away) counts as what its factors make of it.
 __device__ __forceinline__ PolicyRow<double> policy_row_wide(float log_ratio, float q, bool has_ref, double adv, double w, const Policy &p, bool clipped) {
     const double free = -adv * wide_exp(log_ratio);
     const bool small = fabsf(q) < 0.5f;
@@ -290,9 +294,7 @@ __device__ __forceinline__ PolicyRow<double> policy_row_wide(float log_ratio, fl
           : small ? (double)(q * q * (1.f / 2 + q * (1.f / 6 + q * (1.f / 24 + q * (1.f / 120 + q * (1.f / 720 + q * (1.f / 5040 + q * (1.f / 40320))))))))
                   : wide_k(q);
     r.loss = p.kl != 0.f ? r.part + (double)p.kl * r.k : r.part;
-    constexpr double kMost = 0x1.fffffep127;
-    const double c = w * (double)p.scale * ((clipped ? 0.0 : free) - (p.kl != 0.f ? (double)p.kl * e : 0.0));
-    r.c = c > kMost ? kMost : c < -kMost ? -kMost : c;   // (NaN stays)
+    r.c = held_to_f32(w * (double)p.scale * ((clipped ? 0.0 : free) - (p.kl != 0.f ? (double)p.kl * e : 0.0)));
     return r;
 }
 // is the log of the ratio past the border that its advantage's sign puts up?
@@ -876,7 +878,7 @@ template <bool SPLIT> __global__ void __launch_bounds__(1024) preference_pair_ke
         a.seq_logp[2 * pair + 1] = (float)s[1];
     }
     if (!a.coef) return;
-    const float g = (float)((double)a.scale * (double)a.beta * ((double)a.smooth - 1.0 / (1.0 + exp(h))));
+    const float g = (float)held_to_f32((double)a.scale * (double)a.beta * ((double)a.smooth - 1.0 / (1.0 + exp(h))));
     for (int q = 0; q < 2; q++)
         for (long long r = begin[q] + threadIdx.x; r < end[q]; r += 1024) a.coef[r] = q ? -g : g;
 }

@@ -582,7 +582,7 @@ int emadapt_policy_loss(const void *logits, int dtype, int64_t ldl, const int64_
  * device, not decreasing, within [0, M]; a sequence may be empty); sequences 2j and 2j + 1 are the chosen and the rejected one of pair j.
  *   seq_logp[s] = sum of logp over the sequence      h_j = beta ((seq_logp[2j] - ref_logp[2j]) - (seq_logp[2j+1] - ref_logp[2j+1]))
  *   loss[j] = (1 - label_smoothing) softplus(-h_j) + label_smoothing softplus(h_j)
- *   dlogits = grad_scale * d (sum_j loss[j]) / d logits; rows of no sequence: 0
+ *   dlogits = grad_scale * d (sum_j loss[j]) / d logits; rows of no sequence: 0; grad_scale * d loss[j] / d seq_logp is held to f32's range
  * A start outside [0, M] is taken as the nearest bound (nothing outside the rows is touched). */
 size_t emadapt_preference_loss_workspace_bytes(int64_t M, int64_t C);
 int emadapt_preference_loss(const void *logits, int dtype, int64_t ldl, const int64_t *labels, const int64_t *seq_start, int64_t pairs,
